@@ -13,6 +13,9 @@ import os
 import torch
 
 from saelens_b200.ops._build import load as _load
+from saelens_b200.ops.fp8 import gemm_fp8, linear_fp8, quantize_fp8
+from saelens_b200.ops.norms import residual_norm
+from saelens_b200.ops.positions import rotary, rotary_frequencies
 from saelens_b200.ops.status import StatusWord
 
 __all__ = [
@@ -25,6 +28,12 @@ __all__ = [
     "decode_mse",
     "attention",
     "gather_rows",
+    "quantize_fp8",
+    "gemm_fp8",
+    "linear_fp8",
+    "residual_norm",
+    "rotary",
+    "rotary_frequencies",
     "StatusWord",
 ]
 

@@ -41,6 +41,9 @@ SOURCES = [
     "attention.cu",
     "mp.cu",
     "rows.cu",
+    "rotary.cu",
+    "block_norm.cu",
+    "fp8.cu",
 ]
 
 NVCC_FLAGS = [

@@ -1,0 +1,987 @@
+// Matrix product with a frozen weight in 8-bit floating point (e4m3), one scale per block of 128:
+//     y[m, f] = sum over blocks b of  xs[m, b] ws[f / 128, b]  sum over r in b of  xq[m, r] wq[f, r]   (+ bias[f])
+// x is quantised on the way in, one scale for a row's 128 consecutive values:
+//     xs = max(|x|) / 448,   xq = e4m3(448 x / max(|x|))
+// (448 is the largest e4m3 value; the quotient is formed as (7/16 x) / max * 1024, whose numerator
+// is exact for 16-bit x and cannot overflow, so it is rounded once and values on the border of two
+// e4m3 neighbours fall the same way in any arithmetic; the maximum is at least 448 * 2^-126, so that
+// a scale is a normal number; a block with an infinity or NaN makes its whole row NaN).
+// The weight has a scale for each 128 x 128 block.  The gradient of x is the same product with the
+// roles of the weight's sides changed, dx = Q(dy) W: the weight is then read as an MN-major operand,
+// in place.
+//
+// The tensor cores sum one block of 128 exactly scaled alike, in fp32; the scales differ from block
+// to block, so each block's accumulator is read out of tensor memory, scaled and added to fp32 sums
+// in registers while the next block is multiplied into a second accumulator.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp8.h>
+#include <torch/types.h>
+
+#include <algorithm>
+#include <tuple>
+
+#include "check.h"
+#include "common.cuh"
+#include "tmap.h"
+#include "vec.cuh"
+
+namespace sb {
+namespace fp8 {
+
+constexpr int BLK = 128;               // values a scale covers, along the reduction and (weights) the features
+constexpr float MAXV = 448.f;
+constexpr uint32_t LEAST_BITS = 0x04e00000u;  // 448 * 2^-126
+
+// ---------------------------------------------------------------------------------------------
+// quantisation
+// ---------------------------------------------------------------------------------------------
+// Bit patterns of absolute values order like the values, with NaN above infinity: a NaN stays.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ __forceinline__ float quotient(float v, float most) { return v * 0.4375f / most * 1024.f; }
+
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float most) {
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(quotient(v[4 * h], most), quotient(v[4 * h + 1], most)),
+                                                 __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(
+        make_float2(quotient(v[4 * h + 2], most), quotient(v[4 * h + 3], most)), __NV_SATFINITE, __NV_E4M3);
+    w[h] = lo | (hi << 16);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// 8 values from column c of a row; columns from K on are 0.  ALIGNED: rows start on 16 bytes and K is
+// a multiple of 8.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t K, float (&v)[8]) {
+  if (ALIGNED) {
+    vec::Pack<T, 8> p;
+    if (c < K) p.load(row + c);
+    else p.zero();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p.get(j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < K ? vec::to_f<T>(row[c + j]) : 0.f;
+  }
+}
+
+// The largest absolute value (as bits, at least LEAST_BITS) of the 16 lanes of a half-warp.
+__device__ __forceinline__ float half_warp_most(const float (&v)[8]) {
+  uint32_t m = LEAST_BITS;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return __uint_as_float(m);
+}
+
+// Rows: a half-warp quantises a row's 128 values, 8 a lane; 16 rows a block, `per` blocks of 128 a
+// half-warp (at most QPER, all loads issued before the first maximum).  Memory-bound: 2 bytes read
+// and 1 written a value.
+constexpr int QPER = 4;
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int64_t K,
+                                                            uint8_t* __restrict__ q, int64_t ldq,
+                                                            float* __restrict__ scale, int64_t lds, int per) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int lane = threadIdx.x & 15;
+  const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
+  const int64_t kb0 = int64_t(blockIdx.y) * per, KB = (K + BLK - 1) / BLK;
+  float v[QPER][8];
+#pragma unroll
+  for (int i = 0; i < QPER; ++i) {
+    if (i < per && kb0 + i < KB && row < M) {
+      load8<T, ALIGNED>(x + row * ldx, (kb0 + i) * BLK + lane * 8, K, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < QPER; ++i) {
+    if (i >= per) break;  // uniform
+    const float most = half_warp_most(v[i]);
+    const int64_t kb = kb0 + i, c = kb * BLK + lane * 8;
+    if (row < M && kb < KB) {
+      if (c < ldq) *reinterpret_cast<uint2*>(q + row * ldq + c) = quantize8(v[i], most);
+      if (lane == 0) scale[kb * lds + row] = most / MAXV;
+    }
+  }
+}
+
+// Weights: a block of 256 threads quantises one 128 x 128 block, 64 values a thread in registers.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restrict__ x, int64_t ldx, int64_t N, int64_t K,
+                                                              uint8_t* __restrict__ q, int64_t ldq,
+                                                              float* __restrict__ scale) {
+  __shared__ uint32_t red[8];
+  const int64_t kb = blockIdx.x, nb = blockIdx.y;
+  const int64_t c = kb * BLK + (threadIdx.x & 15) * 8;
+  float v[8][8];
+  uint32_t m = LEAST_BITS;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = nb * BLK + i * 16 + (threadIdx.x >> 4);
+    if (row < N) {
+      load8<T, ALIGNED>(x + row * ldx, c, K, v[i]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+  const float most = __uint_as_float(m);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t row = nb * BLK + i * 16 + (threadIdx.x >> 4);
+    if (row < N && c < ldq) *reinterpret_cast<uint2*>(q + row * ldq + c) = quantize8(v[i], most);
+  }
+  if (threadIdx.x == 0) scale[nb * gridDim.x + kb] = most / MAXV;
+}
+
+// ---------------------------------------------------------------------------------------------
+// products
+// ---------------------------------------------------------------------------------------------
+// Instruction descriptor of kind::f8f6f4: e4m3 operands, fp32 accumulator; the bits mark MN-major ones.
+__host__ __device__ constexpr uint32_t make_idesc(int M, int N, bool a_mn, bool b_mn) {
+  return (1u << 4) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t(N >> 3) << 17) |
+         (uint32_t(M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+// 16-byte aligned bulk copy global -> this CTA's shared memory, counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+struct Prod {
+  const void* x;        // fused quantisation: the rows themselves
+  int64_t ldx;
+  const float* xs;      // [blocks of the reduction][ldxs], a row's scale at its index
+  int64_t ldxs;
+  const float* ws;      // scale of (feature block, reduction block) at fb * ws_f + rb * ws_r
+  int64_t ws_f, ws_r;
+  const float* bias;    // [features] or nullptr
+  void* out;            // [M, ldo]
+  int64_t ldo;
+  int M, F, R;          // rows, features, length of the reduction
+  int splits;           // parts of the reduction (the cluster's blocks)
+  int dependent;        // 1: launched while the quantisation before it may still run (not read on the device)
+  int* status;
+};
+
+// ---- few rows -------------------------------------------------------------------------------
+// Up to NT rows.  The weight is the tensor cores' 128-row operand and the rows of x the narrow one, so
+// that no part of the tile is idle weight; the time is the weight's bytes.  A block owns 128
+// features and a part of the reduction; the blocks of a cluster hold the parts of the same features
+// and add their sums over distributed shared memory in block order.  Two blocks share an SM (half
+// its shared memory each): the grid then fills it with finer parts.
+//   warp 0      weight tiles by TMA (and x tiles and scales, unless they are quantised here)
+//   warp 1      tcgen05.mma, 4 a block of 128
+//   warps 2..5  scaled sums in registers: a feature a thread, NT columns
+//   warps 6..9  FUSED: quantise x into the stage's tile, a half-warp for a row's 128 values
+template <int NT>
+struct Few {
+  static constexpr int W_BYTES = BLK * BLK, X_BYTES = NT * BLK, STAGE = W_BYTES + X_BYTES;
+  static constexpr int STAGES = NT <= 16 ? 6 : NT <= 32 ? 5 : 4;
+  static constexpr int RING = STAGES + 2;  // scales outlive their tile by the two accumulators
+  static constexpr int TMEM = 2 * NT < 32 ? 32 : 2 * NT;
+  static constexpr int SMEM = STAGES * STAGE + RING * NT * 4 + 1024 + 512;
+};
+
+template <int NT, bool FUSED, bool ALIGNED, bool W_MN, class TX, class TO>
+__global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                    const __grid_constant__ Prod a) {
+  using C = Few<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sX = smem + C::STAGES * C::W_BYTES;
+  float* sS = reinterpret_cast<float*>(sX + C::STAGES * C::X_BYTES);  // [RING][NT]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sS + C::RING * NT);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* sfull = empty + C::STAGES;
+  uint64_t* tfull = sfull + C::RING;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x % a.splits, fb = blockIdx.x / a.splits;
+  const int RB = (a.R + BLK - 1) / BLK;
+  const int rb0 = int(int64_t(split) * RB / a.splits), n = int(int64_t(split + 1) * RB / a.splits) - rb0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], FUSED ? 1 + a.M : 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < C::RING; ++s) mbar_init(&sfull[s], FUSED ? a.M : 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&tfull[s], 1);
+      mbar_init(&tempty[s], 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::TMEM);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmW);
+    if (!FUSED) tma_prefetch_desc(&tmX);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  float acc[NT];
+#pragma unroll
+  for (int c = 0; c < NT; ++c) acc[c] = 0.f;
+  const int q = warp & 3;
+  const int f = fb * BLK + q * 32 + lane;  // this thread's feature (warps 2..5)
+
+  if (warp == 0) {
+    if (elect_one()) {
+      auto load_w = [&](int j) {
+        const int s = j % C::STAGES, r = (rb0 + j) * BLK;
+        if (W_MN) tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], fb * BLK, r);
+        else tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], r, fb * BLK);
+      };
+      auto load_x = [&](int j) {
+        const int s = j % C::STAGES, g = j % C::RING;
+        tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], (rb0 + j) * BLK, 0);
+        mbar_arrive_expect_tx(&sfull[g], NT * 4);
+        bulk_load(sS + g * NT, a.xs + int64_t(rb0 + j) * a.ldxs, NT * 4, &sfull[g]);
+      };
+      const uint32_t tx = FUSED ? C::W_BYTES : C::STAGE;
+      // the weight does not depend on the kernel that quantises x: its first tiles are on their way
+      // before that kernel ends
+      const int ahead = min(n, C::STAGES);
+      for (int j = 0; j < ahead; ++j) {
+        mbar_arrive_expect_tx(&full[j], tx);
+        load_w(j);
+      }
+      int j = ahead;
+      bool ok = true;
+      if (!FUSED) {
+        grid_dependency_wait();
+        for (int i = 0; i < ahead; ++i) load_x(i);
+      }
+      for (; j < n; ++j) {
+        const int s = j % C::STAGES;
+        if (!mbar_wait_bounded(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
+          ok = false;
+          break;
+        }
+        mbar_arrive_expect_tx(&full[s], tx);
+        load_w(j);
+        if (!FUSED) load_x(j);
+      }
+      if (!ok) {  // the copies in flight land before the block leaves
+        for (int i = max(0, j - C::STAGES); i < j; ++i) {
+          volatile int dummy = 0;
+          mbar_wait_bounded(&full[i % C::STAGES], (i / C::STAGES) & 1, &dummy, nullptr, 0);
+          if (!FUSED) mbar_wait_bounded(&sfull[i % C::RING], (i / C::RING) & 1, &dummy, nullptr, 0);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc(128, NT, W_MN, false);
+      for (int j = 0; j < n; ++j) {
+        const int s = j % C::STAGES, t = j & 1;
+        if (!mbar_wait_bounded(&tempty[t], ((j >> 1) & 1) ^ 1, abort_flag, a.status, kTimeoutMmaTmemEmpty)) break;
+        if (!mbar_wait_bounded(&full[s], (j / C::STAGES) & 1, abort_flag, a.status, kTimeoutMmaFull)) break;
+        tc_fence_after();
+        const uint32_t w = smem_u32(sW + s * C::W_BYTES), x = smem_u32(sX + s * C::X_BYTES);
+#pragma unroll
+        for (int k = 0; k < BLK / 32; ++k)
+          umma_e4m3(tmem + t * NT, W_MN ? make_sdesc_sw128_mnmajor(w + k * 4096, 16384) : make_sdesc_sw128_kmajor(w + k * 32),
+                    make_sdesc_sw128_kmajor(x + k * 32), idesc, k > 0);
+        umma_commit(&empty[s]);
+        umma_commit(&tfull[t]);
+      }
+    }
+    __syncwarp();
+  } else if (warp < 6) {
+    float wv = 0.f;  // lane l: the weight's scale of block (j & ~31) + l
+    for (int j = 0; j < n; ++j) {
+      if ((j & 31) == 0 && j + lane < n) wv = a.ws[fb * a.ws_f + (rb0 + j + lane) * a.ws_r];
+      const float ws = __shfl_sync(0xffffffffu, wv, j & 31);
+      const int t = j & 1, g = j % C::RING;
+      bool ok = mbar_wait_bounded(&sfull[g], (j / C::RING) & 1, abort_flag, a.status, kTimeoutEpilogue);
+      ok = ok && mbar_wait_bounded(&tfull[t], (j >> 1) & 1, abort_flag, a.status, kTimeoutEpilogue);
+      if (!__all_sync(0xffffffffu, ok)) break;  // the warp leaves as one
+      tc_fence_after();
+      uint32_t r[NT];
+#pragma unroll
+      for (int c = 0; c < NT; c += 16) tmem_ld_x16(tmem + (uint32_t(q * 32) << 16) + t * NT + c, r + c);
+      tmem_ld_wait();
+      const float4* xs = reinterpret_cast<const float4*>(sS + g * NT);
+#pragma unroll
+      for (int c = 0; c < NT; c += 4) {
+        const float4 v = xs[c / 4];
+        acc[c] += __uint_as_float(r[c]) * (v.x * ws);
+        acc[c + 1] += __uint_as_float(r[c + 1]) * (v.y * ws);
+        acc[c + 2] += __uint_as_float(r[c + 2]) * (v.z * ws);
+        acc[c + 3] += __uint_as_float(r[c + 3]) * (v.w * ws);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[t]);
+    }
+    __syncwarp();
+  } else if (FUSED) {
+    // item i: 128 values of row i % M of the block's reduction block i / M
+    const int hw = (threadIdx.x - 192) >> 4, l = threadIdx.x & 15;
+    const uint32_t mask = 0xffffu << (lane & 16);
+    const int items = n * a.M;
+    // every half-warp takes part in the warp's shuffles, with or without an item of its own
+    for (int i0 = hw & ~1; i0 < items; i0 += 8) {
+      const int i = i0 + (hw & 1);
+      const bool have = i < items;
+      const int j = have ? i / a.M : 0, m = have ? i - j * a.M : 0;
+      float v[8];
+      load8<TX, ALIGNED>(static_cast<const TX*>(a.x) + m * a.ldx, int64_t(rb0 + j) * BLK + l * 8, have ? a.R : 0, v);
+      const float most = half_warp_most(v);
+      const uint2 w = quantize8(v, most);
+      const int s = j % C::STAGES, g = j % C::RING;
+      bool ok = true;
+      if (have) ok = mbar_wait_bounded(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer);
+      if (have && ok) {
+        // row m of the stage's tile in the 128-byte swizzle: 16-byte granule l / 2 at (l / 2) ^ (m % 8)
+        *reinterpret_cast<uint2*>(sX + s * C::X_BYTES + m * BLK + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8) = w;
+        if (l == 0) sS[g * NT + m] = most / MAXV;
+        fence_proxy_async_smem();
+        __syncwarp(mask);
+        if (l == 0) {
+          mbar_arrive(&full[s]);
+          mbar_arrive(&sfull[g]);
+        }
+      }
+      __syncwarp();
+      if (__any_sync(0xffffffffu, !ok)) break;
+    }
+  }
+
+  auto store = [&](int m, float v) {
+    if (f < a.F) static_cast<TO*>(a.out)[m * a.ldo + f] = vec::from_f<TO>(v + (a.bias ? a.bias[f] : 0.f));
+  };
+  const bool sums = warp >= 2 && warp < 6;
+  if (a.splits == 1) {
+    if (sums)
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+        if (c < a.M) store(c, acc[c]);
+  } else {
+    // every tile of the block has been multiplied: its memory holds the sums for the cluster
+    float* red = reinterpret_cast<float*>(smem);  // [NT][128]
+    if (sums)
+#pragma unroll
+      for (int c = 0; c < NT; ++c) red[c * BLK + q * 32 + lane] = acc[c];
+    cluster_sync_all();
+    if (sums) {
+      const uint32_t mine = smem_u32(red) + uint32_t(q * 32 + lane) * 4;
+      for (int c = split; c < a.M; c += a.splits) {
+        float v = 0.f;
+        for (int p = 0; p < a.splits; ++p) v += ld_cluster_f32(mapa_shared(mine + uint32_t(c) * BLK * 4, uint32_t(p)));
+        store(c, v);
+      }
+    }
+    cluster_sync_all();  // no block leaves while another may read its sums
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM);
+  }
+}
+
+// ---- many rows ------------------------------------------------------------------------------
+// Persistent, one block an SM: tiles of 128 rows by BN features, each block of 128 of the reduction in
+// one of two TMEM accumulators.
+//   warps 0..7  scaled sums in registers: a row a thread, BN / 2 features (warps 0-3 the first half)
+//   warp 8      TMA;  warp 9  tcgen05.mma
+template <int BN>
+struct Many {
+  static constexpr int X_BYTES = 128 * BLK, W_BYTES = BN * BLK, STAGE = X_BYTES + W_BYTES;
+  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int OUT = 32 * 128;  // one warp's staging tile: 32 rows of 128 bytes
+  static constexpr int SMEM = STAGES * STAGE + 8 * OUT + 1024 + 256;
+  static constexpr int GROUP = 4096 / BN;  // feature tiles walked together (L2 reuse)
+};
+
+__device__ __forceinline__ void walk(int t, int num_m, int num_f, int group, int& mt, int& ft) {
+  const int g = t / (num_m * group), first = g * group;
+  const int size = min(group, num_f - first);
+  const int r = t - g * num_m * group;
+  mt = r / size;
+  ft = first + r % size;
+}
+
+// acc (two fp32) += t (two fp32) * s
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s2) {
+  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(s2));
+}
+__device__ __forceinline__ uint64_t both(float s) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(s));
+  return v;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+
+// A warp stores 128 bytes of each of its 32 rows (lane: row `lane`, values v, from column c0 of the
+// tile's feature range) through its staging tile, so that a store instruction covers 4 rows x 128
+// contiguous bytes.  `wide`: rows of out start on 16 bytes.
+template <class TO>
+__device__ __forceinline__ void store_rows(uint8_t* stage, const float* v, TO* out, int64_t ldo, int row0, int M, int c0,
+                                           int F, int lane, bool wide) {
+  constexpr int PER = 16 / int(sizeof(TO));
+#pragma unroll
+  for (int g = 0; g < 8; ++g) {
+    vec::Pack<TO, PER> p;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) p.set(j, v[g * PER + j]);
+    p.store(reinterpret_cast<TO*>(stage + lane * 128 + ((g ^ (lane & 7)) << 4)));
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = i * 4 + (lane >> 3), g = lane & 7;
+    const int row = row0 + r, col = c0 + g * PER;
+    vec::Pack<TO, PER> p;
+    p.load(reinterpret_cast<const TO*>(stage + r * 128 + ((g ^ (r & 7)) << 4)));
+    if (row < M && col < F) {
+      TO* o = out + int64_t(row) * ldo + col;
+      if (wide && col + PER <= F) {
+        p.store(o);
+      } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (col + j < F) o[j] = vec::from_f<TO>(p.get(j));
+      }
+    }
+  }
+  __syncwarp();
+}
+
+template <int BN, bool W_MN, class TO>
+__global__ void __launch_bounds__(320, 1)
+    many_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                     const __grid_constant__ Prod a) {
+  using C = Many<BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sX = smem;
+  uint8_t* sW = smem + C::STAGES * C::X_BYTES;
+  uint8_t* sOut = smem + C::STAGES * C::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 8 * C::OUT);
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* tfull = empty + C::STAGES;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_m = (a.M + 127) / 128, num_f = (a.F + BN - 1) / BN, tiles = num_m * num_f;
+  const int RB = (a.R + BLK - 1) / BLK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&tfull[s], 1);
+      mbar_init(&tempty[s], 8);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_relinquish();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmW);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  if (warp == 8) {
+    if (elect_one()) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int mt, ft;
+        walk(t, num_m, num_f, C::GROUP, mt, ft);
+        for (int rb = 0; rb < RB; ++rb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait_bounded(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], C::STAGE);
+          tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], rb * BLK, mt * 128);
+          if (W_MN) {
+#pragma unroll
+            for (int c = 0; c < BN / 128; ++c)
+              tma_load_2d(sW + s * C::W_BYTES + c * 16384, &tmW, &full[s], ft * BN + c * 128, rb * BLK);
+          } else {
+            tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], rb * BLK, ft * BN);
+          }
+        }
+      }
+      if (!ok) {
+        const uint32_t first = it > C::STAGES ? it - C::STAGES : 0;
+        for (uint32_t j = first; j < it; ++j) {
+          volatile int dummy = 0;
+          mbar_wait_bounded(&full[j % C::STAGES], (j / C::STAGES) & 1, &dummy, nullptr, 0);
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (elect_one()) {
+      constexpr uint32_t idesc = make_idesc(128, BN, false, W_MN);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        for (int rb = 0; rb < RB; ++rb, ++it) {
+          const int s = it % C::STAGES, c = it & 1;
+          if (!mbar_wait_bounded(&tempty[c], ((it >> 1) & 1) ^ 1, abort_flag, a.status, kTimeoutMmaTmemEmpty) ||
+              !mbar_wait_bounded(&full[s], (it / C::STAGES) & 1, abort_flag, a.status, kTimeoutMmaFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t x = smem_u32(sX + s * C::X_BYTES), w = smem_u32(sW + s * C::W_BYTES);
+#pragma unroll
+          for (int k = 0; k < BLK / 32; ++k)
+            umma_e4m3(tmem + c * BN, make_sdesc_sw128_kmajor(x + k * 32),
+                      W_MN ? make_sdesc_sw128_mnmajor(w + k * 4096, 16384) : make_sdesc_sw128_kmajor(w + k * 32), idesc,
+                      k > 0);
+          umma_commit(&empty[s]);
+          umma_commit(&tfull[c]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3, half = warp >> 2;
+    constexpr int COLS = BN / 2;
+    uint8_t* stage = sOut + warp * C::OUT;
+    const bool wide = (a.ldo * int64_t(sizeof(TO))) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int mt, ft;
+      walk(t, num_m, num_f, C::GROUP, mt, ft);
+      const int row0 = mt * 128 + q * 32, row = row0 + lane;
+      const int col0 = ft * BN + half * COLS;
+      // past the last row or feature block the sums are zeros times a scale of 0
+      const float* xs = a.xs + row;
+      const float* ws = a.ws + (col0 / BLK) * a.ws_f;
+      const bool in = row < a.M && col0 < a.F;
+      auto scale = [&](int rb) { return in && rb < RB ? xs[rb * a.ldxs] * ws[rb * a.ws_r] : 0.f; };
+      uint64_t acc[COLS / 2];
+#pragma unroll
+      for (int c = 0; c < COLS / 2; ++c) acc[c] = 0ull;
+      float s0 = scale(0), s1 = scale(1);
+      for (int rb = 0; rb < RB; ++rb, ++it) {
+        const float s2 = scale(rb + 2);
+        const int c = it & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&tfull[c], (it >> 1) & 1, abort_flag, a.status, kTimeoutEpilogue));
+        if (!ok) break;  // the warp leaves as one
+        tc_fence_after();
+        const uint32_t at = tmem + (uint32_t(q * 32) << 16) + c * BN + half * COLS;
+        const uint64_t sc = both(s0);
+#pragma unroll
+        for (int h = 0; h < COLS / 32; ++h) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(at + h * 32, r);
+          tmem_ld_wait();
+          if (h == COLS / 32 - 1) {  // read out: the accumulator is free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[c]);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) fma2(acc[h * 16 + i], r[2 * i], r[2 * i + 1], sc);
+        }
+        s0 = s1;
+        s1 = s2;
+      }
+      if (!ok) break;
+      constexpr int CH = 128 / int(sizeof(TO));  // columns of a staged store
+#pragma unroll
+      for (int c = 0; c < COLS / CH; ++c) {
+        float v[CH];
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) {
+          const float2 p = halves(acc[c * (CH / 2) + i]);
+          v[2 * i] = p.x;
+          v[2 * i + 1] = p.y;
+        }
+        if (a.bias) {
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
+            if (col0 + c * CH + i < a.F) v[i] += __ldg(a.bias + col0 + c * CH + i);
+        }
+        store_rows<TO>(stage, v, static_cast<TO*>(a.out), a.ldo, row0, a.M, col0 + c * CH, a.F, lane, wide);
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 2 * BN);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------
+static int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+static bool rows_aligned(const torch::Tensor& x) {
+  return x.size(1) % 8 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0 &&
+         (x.size(0) <= 1 || (x.stride(0) * x.element_size()) % 16 == 0);
+}
+
+static bool float_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf || t == at::kFloat; }
+
+static void check_rows(const torch::Tensor& x, const char* what) {
+  SB_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1) && float_type(x.scalar_type()), what,
+           ": CUDA bf16, fp16 or fp32 [rows, columns], columns contiguous");
+  SB_CHECK(x.size(1) >= 1 && x.size(0) < (1ll << 31) - 256 && x.size(1) < (1ll << 31) - 256, what, ": size");
+}
+
+template <class T>
+static void quantize_rows_t(const torch::Tensor& x, uint8_t* q, int64_t ldq, float* s, int64_t lds, cudaStream_t st) {
+  const int64_t M = x.size(0), K = x.size(1), KB = (K + BLK - 1) / BLK;
+  const int64_t rb = (M + 15) / 16;
+  // several blocks of 128 a half-warp once there are blocks for every SM without
+  const int per = rb * KB >= 148 * 8 * QPER ? QPER : 1;
+  const int64_t ny = (KB + per - 1) / per;
+  SB_CHECK(ny <= 65535, "quantize_fp8: rows of more than 8 million values");
+  const dim3 grid{unsigned(rb), unsigned(ny)};
+  const T* p = static_cast<const T*>(x.data_ptr());
+  if (rows_aligned(x)) quantize_rows_kernel<T, true><<<grid, 256, 0, st>>>(p, x.stride(0), M, K, q, ldq, s, lds, per);
+  else quantize_rows_kernel<T, false><<<grid, 256, 0, st>>>(p, x.stride(0), M, K, q, ldq, s, lds, per);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+static void quantize_rows(const torch::Tensor& x, uint8_t* q, int64_t ldq, float* s, int64_t lds, cudaStream_t st) {
+  if (x.scalar_type() == at::kBFloat16) quantize_rows_t<__nv_bfloat16>(x, q, ldq, s, lds, st);
+  else if (x.scalar_type() == at::kHalf) quantize_rows_t<__half>(x, q, ldq, s, lds, st);
+  else quantize_rows_t<float>(x, q, ldq, s, lds, st);
+}
+
+template <class T>
+static void quantize_blocks_t(const torch::Tensor& x, uint8_t* q, int64_t ldq, float* s, cudaStream_t st) {
+  const int64_t N = x.size(0), K = x.size(1);
+  const int64_t nb = (N + BLK - 1) / BLK;
+  SB_CHECK(nb <= 65535, "quantize_fp8: more than 8 million rows");
+  const dim3 grid{unsigned((K + BLK - 1) / BLK), unsigned(nb)};
+  const T* p = static_cast<const T*>(x.data_ptr());
+  if (rows_aligned(x)) quantize_blocks_kernel<T, true><<<grid, 256, 0, st>>>(p, x.stride(0), N, K, q, ldq, s);
+  else quantize_blocks_kernel<T, false><<<grid, 256, 0, st>>>(p, x.stride(0), N, K, q, ldq, s);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// The weight as the product reads it: features F, reduction R, and where its scales lie.
+struct Weight {
+  const void* q;
+  int64_t ld, F, R;
+  bool mn;  // stored [R, F]: the gradient's product
+  const float* ws;
+  int64_t ws_f, ws_r;
+};
+
+static Weight weight_of(const torch::Tensor& w, const torch::Tensor& s, bool transposed) {
+  SB_CHECK(w.is_cuda() && w.dim() == 2 && w.scalar_type() == at::kFloat8_e4m3fn && (w.size(1) <= 1 || w.stride(1) == 1),
+           "fp8 product: the weight must be CUDA e4m3 [features, width], width contiguous");
+  const int64_t N = w.size(0), K = w.size(1);
+  SB_CHECK(N >= 1 && K >= 1 && N < (1ll << 31) - 256 && K < (1ll << 31) - 256, "fp8 product: size of the weight");
+  const int64_t ld = N > 1 ? w.stride(0) : up(K, 16);
+  SB_CHECK(ld % 16 == 0 && ld >= K && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0,
+           "fp8 product: rows of the weight must start on 16 bytes (quantize_fp8 lays them out so)");
+  const int64_t NB = (N + BLK - 1) / BLK, KB = (K + BLK - 1) / BLK;
+  SB_CHECK(s.device() == w.device() && s.scalar_type() == at::kFloat && s.dim() == 2 && s.size(0) == NB && s.size(1) == KB,
+           "fp8 product: the weight's scales must be fp32 [", NB, ", ", KB, "]");
+  Weight r{};
+  r.q = w.data_ptr();
+  r.ld = ld;
+  r.mn = transposed;
+  r.F = transposed ? K : N;
+  r.R = transposed ? N : K;
+  r.ws = s.data_ptr<float>();
+  r.ws_f = transposed ? s.stride(1) : s.stride(0);
+  r.ws_r = transposed ? s.stride(0) : s.stride(1);
+  return r;
+}
+
+static CUtensorMap weight_map(const Weight& w, int box_features) {
+  // box: 128 along the stored row by 128 (or the tile's features) rows
+  const int64_t rows = w.mn ? w.R : w.F, cols = w.mn ? w.F : w.R;
+  return make_tmap_2d(w.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, rows, cols, w.ld, w.mn ? BLK : box_features, BLK,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <class K>
+static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st,
+                   const CUtensorMap& tW, const CUtensorMap& tX, const Prod& a) {
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (dependent) {  // may start while the kernel before it (the quantisation) still runs
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tW, tX, a));
+}
+
+constexpr int FEW = 64;         // rows up to which the few-rows kernel runs
+constexpr int FUSED_ROWS = 16;  // rows up to which it quantises them itself
+
+// Parts of the reduction: so many that two blocks for every SM are running, 8 at most.
+static int splits_for(int64_t feature_tiles, int64_t reduction_blocks, int sms) {
+  const int64_t s = (2 * sms) / feature_tiles;
+  return int(std::max<int64_t>(1, std::min<int64_t>({s, 8, reduction_blocks})));
+}
+
+template <int NT, bool FUSED, class TX, class TO>
+static void few_rows(const Weight& w, const CUtensorMap& tX, Prod a, bool x_aligned, cudaStream_t st) {
+  const int64_t tiles = (w.F + BLK - 1) / BLK;
+  a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+  const dim3 grid{unsigned(tiles * a.splits)};
+  const CUtensorMap tW = weight_map(w, BLK);
+  const int threads = FUSED ? 320 : 192, smem = Few<NT>::SMEM;
+  auto go = [&](auto kern) { launch(kern, grid, threads, smem, a.splits, a.dependent, st, tW, tX, a); };
+  if constexpr (FUSED) {
+    if (!x_aligned) {
+      if (w.mn) go(few_rows_kernel<NT, true, false, true, TX, TO>);
+      else go(few_rows_kernel<NT, true, false, false, TX, TO>);
+      return;
+    }
+  }
+  if (w.mn) go(few_rows_kernel<NT, FUSED, true, true, TX, TO>);
+  else go(few_rows_kernel<NT, FUSED, true, false, TX, TO>);
+}
+
+template <int BN, class TO>
+static void many_rows(const Weight& w, const CUtensorMap& tX, const Prod& a, cudaStream_t st) {
+  const int64_t tiles = ((a.M + 127) / 128) * ((w.F + BN - 1) / BN);
+  SB_CHECK(tiles < (1ll << 31), "fp8 product: too many tiles");
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  const dim3 grid{unsigned(std::min<int64_t>(tiles, sms))};
+  const CUtensorMap tW = weight_map(w, BN);
+  if (w.mn) launch(many_rows_kernel<BN, true, TO>, grid, 320, Many<BN>::SMEM, 1, a.dependent, st, tW, tX, a);
+  else launch(many_rows_kernel<BN, false, TO>, grid, 320, Many<BN>::SMEM, 1, a.dependent, st, tW, tX, a);
+}
+
+// Quantised rows (uint8 [M, R] with row stride ldq, scales [blocks][lds]) times the weight.
+template <class TO>
+static void product(const uint8_t* q, int64_t ldq, const Weight& w, const Prod& a, cudaStream_t st) {
+  const int box = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= FEW ? 64 : 128;
+  const CUtensorMap tX = make_tmap_2d(q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, w.R, ldq, box, BLK, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (a.M <= 16) few_rows<16, false, float, TO>(w, tX, a, true, st);
+  else if (a.M <= 32) few_rows<32, false, float, TO>(w, tX, a, true, st);
+  else if (a.M <= FEW) few_rows<64, false, float, TO>(w, tX, a, true, st);
+  else {
+    const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    const int64_t m = (a.M + 127) / 128;
+    const int64_t wide_tiles = m * ((w.F + 255) / 256);
+    if (wide_tiles >= sms) many_rows<256, TO>(w, tX, a, st);
+    else many_rows<128, TO>(w, tX, a, st);
+  }
+}
+
+static Prod prod_of(const Weight& w, int64_t M, const c10::optional<torch::Tensor>& bias, const torch::Tensor& out,
+                    const torch::Tensor& status, const torch::Tensor& weight) {
+  SB_CHECK(out.device() == weight.device() && out.dim() == 2 && out.size(0) == M && out.size(1) == w.F &&
+               (w.F <= 1 || out.stride(1) == 1) && float_type(out.scalar_type()),
+           "fp8 product: out must be bf16, fp16 or fp32 [rows, features] on the weight's device");
+  if (bias)
+    SB_CHECK(bias->device() == weight.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 &&
+                 bias->size(0) == w.F && bias->is_contiguous(),
+             "fp8 product: bias must be contiguous fp32 [features]");
+  SB_CHECK(status.device() == weight.device() && status.scalar_type() == at::kInt && status.numel() >= 1, "fp8 product: status word");
+  Prod a{};
+  a.ws = w.ws;
+  a.ws_f = w.ws_f;
+  a.ws_r = w.ws_r;
+  a.bias = bias ? bias->data_ptr<float>() : nullptr;
+  a.out = out.data_ptr();
+  a.ldo = M > 1 ? out.stride(0) : w.F;
+  a.M = int(M);
+  a.F = int(w.F);
+  a.R = int(w.R);
+  a.status = status.data_ptr<int>();
+  return a;
+}
+
+template <class T>
+static void linear_t(const torch::Tensor& x, const Weight& w, Prod a, cudaStream_t st) {
+  if (a.M <= FUSED_ROWS) {
+    a.x = x.data_ptr();
+    a.ldx = x.stride(0);
+    few_rows<16, true, T, T>(w, CUtensorMap{}, a, rows_aligned(x), st);
+    return;
+  }
+  const int64_t ldq = up(w.R, 16), lds = up(a.M, 64), RB = (w.R + BLK - 1) / BLK;
+  torch::Tensor q = torch::empty({a.M * ldq}, x.options().dtype(at::kByte));
+  torch::Tensor s = torch::empty({RB * lds}, x.options().dtype(at::kFloat));
+  quantize_rows(x, q.data_ptr<uint8_t>(), ldq, s.data_ptr<float>(), lds, st);
+  a.xs = s.data_ptr<float>();
+  a.ldxs = lds;
+  a.dependent = 1;  // the quantisation itself began after everything before it had ended
+  product<T>(q.data_ptr<uint8_t>(), ldq, w, a, st);
+}
+
+}  // namespace fp8
+
+// e4m3 values and scales of x [rows, columns]: `block_rows` 1 gives a scale for each row's 128
+// columns, 128 one for each 128 x 128 block.  The values' rows start on 16 bytes; row scales come
+// back as a [rows, blocks] view of column-major storage.
+std::tuple<torch::Tensor, torch::Tensor> quantize_fp8(const torch::Tensor& x, int64_t block_rows) {
+  fp8::check_rows(x, "quantize_fp8");
+  SB_CHECK(block_rows == 1 || block_rows == fp8::BLK, "quantize_fp8: block_rows must be 1 or 128, got ", block_rows);
+  const at::cuda::CUDAGuard guard(x.device());
+  auto st = at::cuda::getCurrentCUDAStream();
+  const int64_t M = x.size(0), K = x.size(1), KB = (K + fp8::BLK - 1) / fp8::BLK, ldq = fp8::up(K, 16);
+  torch::Tensor q = torch::empty({M, ldq}, x.options().dtype(at::kByte));
+  uint8_t* qp = q.data_ptr<uint8_t>();
+  torch::Tensor s;
+  if (block_rows == 1) {
+    const int64_t lds = fp8::up(M, 64);
+    torch::Tensor store = torch::empty({KB, lds}, x.options().dtype(at::kFloat));
+    if (M) fp8::quantize_rows(x, qp, ldq, store.data_ptr<float>(), lds, st);
+    s = store.t().narrow(0, 0, M);
+  } else {
+    s = torch::empty({(M + fp8::BLK - 1) / fp8::BLK, KB}, x.options().dtype(at::kFloat));
+    float* sp = s.data_ptr<float>();
+    if (M == 0) {
+    } else if (x.scalar_type() == at::kBFloat16) fp8::quantize_blocks_t<__nv_bfloat16>(x, qp, ldq, sp, st);
+    else if (x.scalar_type() == at::kHalf) fp8::quantize_blocks_t<__half>(x, qp, ldq, sp, st);
+    else fp8::quantize_blocks_t<float>(x, qp, ldq, sp, st);
+  }
+  return {q.narrow(1, 0, K).view(at::kFloat8_e4m3fn), s};
+}
+
+// out = quantised x times the weight (transposed: the product over the weight's rows, the gradient
+// of x), plus bias.  x [rows, R] bf16, fp16 or fp32; weight e4m3 [N, K], scales [N / 128, K / 128].
+void linear_fp8(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& scale,
+                const c10::optional<torch::Tensor>& bias, bool transposed, const torch::Tensor& out,
+                const torch::Tensor& status) {
+  fp8::check_rows(x, "linear_fp8");
+  const fp8::Weight w = fp8::weight_of(weight, scale, transposed);
+  SB_CHECK(x.device() == weight.device() && x.size(1) == w.R, "linear_fp8: x must be [rows, ", w.R, "] on the weight's device");
+  SB_CHECK(out.scalar_type() == x.scalar_type(), "linear_fp8: out must have x's type");
+  const fp8::Prod a = fp8::prod_of(w, x.size(0), bias, out, status, weight);
+  if (a.M == 0) return;
+  const at::cuda::CUDAGuard guard(x.device());
+  auto st = at::cuda::getCurrentCUDAStream();
+  if (x.scalar_type() == at::kBFloat16) fp8::linear_t<__nv_bfloat16>(x, w, a, st);
+  else if (x.scalar_type() == at::kHalf) fp8::linear_t<__half>(x, w, a, st);
+  else fp8::linear_t<float>(x, w, a, st);
+}
+
+// The same for rows that are quantised already: a e4m3 [rows, K], its scales [rows, K / 128] with
+// stride 1 between rows (quantize_fp8's).
+void gemm_fp8(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& weight,
+              const torch::Tensor& scale, const c10::optional<torch::Tensor>& bias, const torch::Tensor& out,
+              const torch::Tensor& status) {
+  const fp8::Weight w = fp8::weight_of(weight, scale, false);
+  const int64_t M = a.dim() == 2 ? a.size(0) : 0, RB = (w.R + fp8::BLK - 1) / fp8::BLK;
+  SB_CHECK(a.device() == weight.device() && a.dim() == 2 && a.scalar_type() == at::kFloat8_e4m3fn && a.size(1) == w.R &&
+               (w.R <= 1 || a.stride(1) == 1) && M < (1ll << 31) - 256,
+           "gemm_fp8: a must be e4m3 [rows, ", w.R, "] on the weight's device, columns contiguous");
+  const int64_t ldq = M > 1 ? a.stride(0) : fp8::up(w.R, 16);
+  SB_CHECK(ldq % 16 == 0 && ldq >= w.R && reinterpret_cast<uintptr_t>(a.data_ptr()) % 16 == 0,
+           "gemm_fp8: rows of a must start on 16 bytes (quantize_fp8 lays them out so)");
+  SB_CHECK(a_scale.device() == a.device() && a_scale.scalar_type() == at::kFloat && a_scale.dim() == 2 &&
+               a_scale.size(0) == M && a_scale.size(1) == RB && (M <= 1 || a_scale.stride(0) == 1),
+           "gemm_fp8: a's scales must be fp32 [", M, ", ", RB, "] with stride 1 between rows");
+  fp8::Prod p = fp8::prod_of(w, M, bias, out, status, weight);
+  if (M == 0) return;
+  // the few-rows kernel copies the scales of a whole row tile at once, in 16-byte units
+  const int64_t tile = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+  p.ldxs = RB > 1 ? a_scale.stride(1) : fp8::up(M, 64);
+  const int64_t room = int64_t(a_scale.storage().nbytes() / sizeof(float)) - a_scale.storage_offset();
+  SB_CHECK(M > fp8::FEW || (p.ldxs % 4 == 0 && reinterpret_cast<uintptr_t>(a_scale.data_ptr()) % 16 == 0 &&
+                            (RB - 1) * p.ldxs + tile <= room),
+           "gemm_fp8: a's scales must be laid out as quantize_fp8 does");
+  p.xs = a_scale.data_ptr<float>();
+  const at::cuda::CUDAGuard guard(a.device());
+  auto st = at::cuda::getCurrentCUDAStream();
+  const uint8_t* q = static_cast<const uint8_t*>(a.data_ptr());
+  if (out.scalar_type() == at::kBFloat16) fp8::product<__nv_bfloat16>(q, ldq, w, p, st);
+  else if (out.scalar_type() == at::kHalf) fp8::product<__half>(q, ldq, w, p, st);
+  else fp8::product<float>(q, ldq, w, p, st);
+}
+
+}  // namespace sb
