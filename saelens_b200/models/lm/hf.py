@@ -152,6 +152,14 @@ def _cfg_from_hf(hc: Any) -> LMConfig:
         eps=getattr(hc, "rms_norm_eps", 1e-6), tie_embeddings=bool(getattr(hc, "tie_word_embeddings", False)),
         model_name=getattr(hc, "_name_or_path", mt) or mt, dtype="float32",
     )
+    rope = dict(getattr(hc, "rope_scaling", None) or getattr(hc, "rope_parameters", None) or {})
+    if (rope.get("rope_type") or rope.get("type")) in ("linear", "dynamic", "llama3", "yarn"):
+        if (rope.get("rope_type") or rope.get("type")) == "dynamic":
+            rope["original_max_position_embeddings"] = kw["n_ctx"]
+        kw["rope_scaling"] = {k: v for k, v in rope.items() if v is not None}
+    part = rope.get("partial_rotary_factor") or getattr(hc, "partial_rotary_factor", None) or 1.0
+    if part != 1.0:
+        kw["rotary_dim"] = int(kw["d_head"] * part)
     if mt in ("qwen2",):
         kw.update(architecture="qwen2", qkv_bias=True)
     elif mt in ("gemma2",):
@@ -166,7 +174,8 @@ def _cfg_from_hf(hc: Any) -> LMConfig:
 
 
 @torch.no_grad()
-def hooked_lm_from_hf(hf_model: nn.Module, dtype: str | None = None, device: Any = None) -> HookedLM:
+def hooked_lm_from_hf(hf_model: nn.Module, dtype: str | None = None, device: Any = None,
+                      weight_quantization: str | None = None) -> HookedLM:
     hc = hf_model.config
     cfg = _cfg_from_hf(hc)
     if dtype is not None:
@@ -222,5 +231,7 @@ def hooked_lm_from_hf(hf_model: nn.Module, dtype: str | None = None, device: Any
         lm.to(getattr(torch, dtype))
     if device is not None:
         lm.to(device)
+    if weight_quantization is not None:
+        lm.quantize_weights(weight_quantization)
     lm.setup()
     return lm

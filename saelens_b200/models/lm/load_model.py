@@ -2,7 +2,8 @@
 
 * "HookedTransformer" / "HookedLM" / "HookedSAETransformer": this package's `HookedLM`; a preset
   name (e.g. "gpt2", "meta-llama/Meta-Llama-3-8B") gives a random-init model of that shape, a local
-  Hugging Face checkpoint directory is converted weight for weight.
+  Hugging Face checkpoint directory is converted weight for weight.  `weight_quantization="fp8"`
+  among the kwargs holds the blocks' projections in 8 bits (`models/lm/fp8.py`).
 * "VLLMModel": the reference's vLLM activation producer (sae_lens/vllm_model.py:548).  Here it is
   this package's producer, `HookedLM`, resolved like "HookedTransformer": it runs to the hooked
   layer on the framework's own kernels (tcgen05 GEMMs and attention).  vLLM engine options
@@ -70,7 +71,7 @@ def load_model(model_class_name: str, model_name: str, device: str | torch.devic
             from saelens_b200.models.lm.hf import hooked_lm_from_hf
 
             hf = AutoModelForCausalLM.from_pretrained(model_name, local_files_only=True)
-            lm = hooked_lm_from_hf(hf, dtype=dtype, device=device)
+            lm = hooked_lm_from_hf(hf, dtype=dtype, device=device, weight_quantization=kw.get("weight_quantization"))
             if cls is not HookedLM:
                 lm.__class__ = cls
                 cls._init_sae_state(lm)

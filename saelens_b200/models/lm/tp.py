@@ -66,6 +66,8 @@ def shard_lm_tensor_parallel(model: Any, group: dist.ProcessGroup, sync_from_roo
     """Shard `model` (a HookedLM) in place for tensor parallelism over `group`; returns the model.
     With `sync_from_root` the group's first rank's weights are broadcast first, so members that
     initialised the model independently (random init) still shard one model."""
+    if any(blk.attn.qkv_fp8 is not None for blk in model.blocks):
+        raise ValueError("shard the model before its weights are quantised")
     ctx = TPContext(group)
     if sync_from_root:
         root = dist.get_global_rank(group, 0)

@@ -63,6 +63,12 @@ class LMConfig:
     attn_softcap: float | None = None
     final_softcap: float | None = None
     query_pre_attn_scalar: float | None = None
+    rotary_dim: int | None = None          # channels of a head that turn (None: all)
+    rotary_interleaved: bool = False       # pairs of neighbours instead of the two halves
+    rope_scaling: dict[str, Any] | None = None  # stretched context, see ops.rotary_frequencies
+    residual_scale: float = 1.0            # what each sub-block adds is multiplied by this
+    branch_gate: bool = False              # and by a learned gate per channel
+    weight_quantization: str | None = None  # "fp8": the blocks' projections in e4m3 (models/lm/fp8.py)
     model_name: str = "custom"
     dtype: str = "bfloat16"
     init_std: float = 0.02
@@ -74,6 +80,10 @@ class LMConfig:
             self.n_key_value_heads = self.n_heads
         if self.n_heads % self.n_key_value_heads:
             raise ValueError("n_heads must be a multiple of n_key_value_heads")
+        if self.weight_quantization not in (None, "fp8"):
+            raise ValueError(f"weight_quantization must be None or 'fp8', got {self.weight_quantization!r}")
+        if self.rotary_dim is not None and not (2 <= self.rotary_dim <= self.d_head and self.rotary_dim % 2 == 0):
+            raise ValueError(f"rotary_dim must be even and from 2 to d_head ({self.d_head}), got {self.rotary_dim}")
 
     def to_dict(self) -> dict[str, Any]:
         return asdict(self)
@@ -280,6 +290,26 @@ class Norm(nn.Module):
         return self.hook_normalized(y.to(x.dtype))
 
 
+def _unwatched(m: nn.Module) -> bool:
+    """Whether no hook of any kind watches the module."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+
+
+def _plain(hook: nn.Module) -> bool:
+    """Whether a hook point passes its tensor on unread (an SAE spliced in its place does not)."""
+    return isinstance(hook, HookPoint) and _unwatched(hook)
+
+
+def _fuses_residual(x: torch.Tensor, out: torch.Tensor, post: Norm | None, hook_out: nn.Module, hook_stream: nn.Module,
+                    then: Norm, cfg: LMConfig) -> bool:
+    """Whether one kernel may do the residual update and the norms around it: inference on CUDA in a
+    type that the single norms run on, nothing reading in between."""
+    return (_native_ok(x) and x.dtype in (torch.bfloat16, torch.float32) and out.dtype == x.dtype == then.w.dtype
+            and 8 <= cfg.d_model <= 16384 and cfg.d_model % 8 == 0 and _plain(hook_out) and _plain(hook_stream)
+            and _unwatched(then)
+            and (post is None or (post.w.dtype == x.dtype and _unwatched(post) and _plain(post.hook_normalized))))
+
+
 def _act(name: str, x: torch.Tensor) -> torch.Tensor:
     if name == "silu":
         return F.silu(x)
@@ -314,6 +344,35 @@ def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1).to(x.dtype)
 
 
+@dataclass
+class RotaryFrequencies:
+    """Rotary positions by their frequencies (partial, interleaved or stretched ones): what
+    `ops.rotary` takes."""
+
+    freq: torch.Tensor  # fp64 [rot / 2]
+    factor: float
+    interleaved: bool
+
+    def turn(self, q: torch.Tensor, k: torch.Tensor, inplace: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+        """q and k [B, S, heads, d] at positions 0 .. S - 1."""
+        if q.is_cuda and not FORCE_TORCH and q.dtype in (torch.bfloat16, torch.float16, torch.float32):
+            from saelens_b200 import ops
+
+            if ops.available():
+                return ops.rotary(q, k, self.freq, interleaved=self.interleaved, factor=self.factor, inplace=inplace)  # type: ignore[return-value]
+        angle = torch.outer(torch.arange(q.shape[1], device=q.device, dtype=torch.float64), self.freq)[None, :, None]
+        cos, sin = (torch.cos(angle) * self.factor).float(), (torch.sin(angle) * self.factor).float()
+        return self._turn_one(q, cos, sin), self._turn_one(k, cos, sin)
+
+    def _turn_one(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+        n = self.freq.shape[0]
+        xf = x.float()
+        a, b = (xf[..., 0 : 2 * n : 2], xf[..., 1 : 2 * n : 2]) if self.interleaved else (xf[..., :n], xf[..., n : 2 * n])
+        a, b = a * cos - b * sin, b * cos + a * sin
+        y = torch.stack((a, b), dim=-1).flatten(-2) if self.interleaved else torch.cat((a, b), dim=-1)
+        return torch.cat((y, xf[..., 2 * n :]), dim=-1).to(x.dtype)
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: LMConfig, dtype: torch.dtype):
         super().__init__()
@@ -329,6 +388,7 @@ class Attention(nn.Module):
         self.hook_rot_q, self.hook_rot_k = HookPoint(), HookPoint()
         self.scale = 1.0 / math.sqrt(cfg.query_pre_attn_scalar if cfg.query_pre_attn_scalar else dh)
         self._qkv = _FusedWeights()
+        self.qkv_fp8: Any = None  # the three projections' 8-bit weight (models/lm/fp8.py)
         # tensor parallelism (models/lm/tp.py): this rank's heads and the group
         self.n_heads_local, self.n_kv_local = H, KV
         self.tp: Any = None
@@ -342,14 +402,19 @@ class Attention(nn.Module):
             return hp(t)
         return self.tp.hooked(hp, t, dim)
 
-    def forward(self, x: torch.Tensor, rot: tuple[torch.Tensor, torch.Tensor] | None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor,
+                rot: tuple[torch.Tensor, torch.Tensor] | RotaryFrequencies | None) -> torch.Tensor:
         B, S, _ = x.shape
         H, KV, dh = self.n_heads_local, self.n_kv_local, self.cfg.d_head
         fused = (x.dtype == torch.bfloat16 and self.q.weight.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0
                  and _native_ok(x))
-        if fused:
+        if fused or self.qkv_fp8 is not None:
             # one GEMM for q, k and v; the heads are strided views of its output
-            qkv = _fused_linear(x, self._qkv, [self.q, self.k, self.v])
+            if self.qkv_fp8 is not None:
+                qkv = self.qkv_fp8(x)
+                fused = qkv.dtype == torch.bfloat16 and _native_ok(qkv)
+            else:
+                qkv = _fused_linear(x, self._qkv, [self.q, self.k, self.v])
             q = self._hook(self.hook_q, qkv[..., : H * dh].view(B, S, H, dh), 2)
             k = self._hook(self.hook_k, qkv[..., H * dh : (H + KV) * dh].view(B, S, KV, dh), 2)
             v = self._hook(self.hook_v, qkv[..., (H + KV) * dh :].view(B, S, KV, dh), 2)
@@ -357,7 +422,12 @@ class Attention(nn.Module):
             q = self._hook(self.hook_q, self.q(x).view(B, S, H, dh), 2)
             k = self._hook(self.hook_k, self.k(x).view(B, S, KV, dh), 2)
             v = self._hook(self.hook_v, self.v(x).view(B, S, KV, dh), 2)
-        if rot is not None:
+        if isinstance(rot, RotaryFrequencies):
+            # nothing else holds the fused projection's output where q and k have no hooks
+            in_place = fused and not (self.hook_q.has_hooks or self.hook_k.has_hooks)
+            q, k = rot.turn(q, k, inplace=in_place)
+            q, k = self._hook(self.hook_rot_q, q, 2), self._hook(self.hook_rot_k, k, 2)
+        elif rot is not None:
             in_place = (fused and rot[0].dtype == torch.float32 and not (self.hook_q.has_hooks or self.hook_k.has_hooks)
                         and q.stride(-1) == 1 and k.stride(-1) == 1)
             if in_place:
@@ -420,6 +490,7 @@ class MLP(nn.Module):
         self.hook_pre = HookPoint()
         self.hook_post = HookPoint()
         self._gate_up = _FusedWeights()
+        self.gate_up_fp8: Any = None  # the two projections' 8-bit weight (models/lm/fp8.py)
         self.d_mlp_local = cfg.d_mlp
         self.tp: Any = None
         self.down_bias_after: torch.Tensor | None = None
@@ -442,12 +513,20 @@ class MLP(nn.Module):
         if self.gated:
             kind = {"silu": 0, "gelu_new": 1, "gelu_pytorch_tanh": 1}.get(self.cfg.act_fn)
             d = self.d_mlp_local
-            if (kind is not None and x.dtype == torch.bfloat16 and self.gate.weight.dtype == torch.bfloat16
+            if self.gate_up_fp8 is not None and not (kind is not None and x.dtype == torch.bfloat16 and d % 8 == 0 and _native_ok(x)):
+                gu = self.gate_up_fp8(x)
+                pre = self._hook(self.hook_pre, gu[..., :d])
+                return self._down(self._hook(self.hook_post, _act(self.cfg.act_fn, pre) * gu[..., d:]))
+            if self.gate_up_fp8 is not None or (
+                    kind is not None and x.dtype == torch.bfloat16 and self.gate.weight.dtype == torch.bfloat16
                     and x.shape[-1] % 8 == 0 and d % 8 == 0 and _native_ok(x)):
                 # one GEMM for the gate and up projections; the activation reads both halves in place
                 from saelens_b200.ops import native
 
-                gu = _fused_linear(x, self._gate_up, [self.gate, self.up])
+                if self.gate_up_fp8 is not None:
+                    gu = self.gate_up_fp8(x)
+                else:
+                    gu = _fused_linear(x, self._gate_up, [self.gate, self.up])
                 pre = self._hook(self.hook_pre, gu[..., :d])
                 up = gu[..., d:]
                 if pre.shape == up.shape and pre.stride(-1) == 1:
@@ -480,24 +559,52 @@ class Block(nn.Module):
         if cfg.sandwich_norm:
             self.ln1_post = Norm(cfg, dtype)
             self.ln2_post = Norm(cfg, dtype)
+        if cfg.branch_gate:
+            self.attn_gate = nn.Parameter(torch.ones(cfg.d_model, dtype=dtype))
+            self.mlp_gate = nn.Parameter(torch.ones(cfg.d_model, dtype=dtype))
         self.hook_resid_pre = HookPoint()
         self.hook_attn_out = HookPoint()
         self.hook_resid_mid = HookPoint()
         self.hook_mlp_out = HookPoint()
         self.hook_resid_post = HookPoint()
 
-    def forward(self, x: torch.Tensor, rot: tuple[torch.Tensor, torch.Tensor] | None) -> torch.Tensor:
+    def _join(self, x: torch.Tensor, out: torch.Tensor, post: Norm | None, gate: torch.Tensor | None, hook_out: nn.Module,
+              hook_stream: nn.Module, then: Norm | None) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """The residual stream after a sub-block's output `out`, and that stream normalised by `then` (the
+        norm that reads it next) where one kernel computes both.  A hook that reads a value in
+        between, or may change the stream, gets the steps one by one; they give the same bits."""
+        cfg = self.cfg
+        if then is not None and _fuses_residual(x, out, post, hook_out, hook_stream, then, cfg):
+            from saelens_b200 import ops
+
+            stream, normed = ops.residual_norm(
+                x, out, then.w, then.b, kind="rms" if then.rms else "layer", eps=then.eps, one_plus=then.one_plus,
+                post_weight=None if post is None else post.w, post_bias=None if post is None else post.b,
+                gate=gate, scale=cfg.residual_scale, round_branch=True)
+            return stream, normed
+        if post is not None:
+            out = post(out)
+        if gate is not None or cfg.residual_scale != 1.0:
+            scaled = out.float() if gate is None else out.float() * gate.float()
+            out = (scaled * cfg.residual_scale).to(out.dtype)
+        out = hook_out(out)
+        return hook_stream(x + out), None
+
+    def forward(self, x: torch.Tensor, rot: tuple[torch.Tensor, torch.Tensor] | RotaryFrequencies | None,
+                normed: torch.Tensor | None = None,
+                then: Norm | None = None) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor | None]:
+        """x -> the stream after the block; with `then`, also that stream normalised by `then` where the
+        block's last kernel computed it (None otherwise).  `normed`: ln1's output, where the kernel
+        before did."""
+        sandwich, gated = self.cfg.sandwich_norm, self.cfg.branch_gate
         x = self.hook_resid_pre(x)
-        a = self.attn(self.ln1(x), rot)
-        if self.cfg.sandwich_norm:
-            a = self.ln1_post(a)
-        a = self.hook_attn_out(a)
-        x = self.hook_resid_mid(x + a)
-        m = self.mlp(self.ln2(x))
-        if self.cfg.sandwich_norm:
-            m = self.ln2_post(m)
-        m = self.hook_mlp_out(m)
-        return self.hook_resid_post(x + m)
+        a = self.attn(self.ln1(x) if normed is None else self.ln1.hook_normalized(normed), rot)
+        x, normed = self._join(x, a, self.ln1_post if sandwich else None, self.attn_gate if gated else None,
+                               self.hook_attn_out, self.hook_resid_mid, self.ln2)
+        m = self.mlp(self.ln2(x) if normed is None else self.ln2.hook_normalized(normed))
+        x, normed = self._join(x, m, self.ln2_post if sandwich else None, self.mlp_gate if gated else None,
+                               self.hook_mlp_out, self.hook_resid_post, then)
+        return x if then is None else (x, normed)
 
 
 class HookedLM(HookedRootModule):
@@ -520,10 +627,13 @@ class HookedLM(HookedRootModule):
             self.unembed = None if cfg.tie_embeddings else NativeLinear(cfg.d_model, cfg.d_vocab, False, dtype)
             self.tokenizer = tokenizer
             self._rot: tuple[torch.Tensor, torch.Tensor] | None = None
+            self._freq: tuple[Any, RotaryFrequencies] | None = None
             if init:
                 self.init_weights()
         if device is not None:
             self.to(device)
+        if init and cfg.weight_quantization is not None:
+            self.quantize_weights(cfg.weight_quantization)
         self.setup()
 
     # ---------------------------------------------------------------- construction
@@ -544,6 +654,17 @@ class HookedLM(HookedRootModule):
             elif name.endswith(".b") or name.endswith("bias"):
                 p.zero_()
 
+    def quantize_weights(self, kind: str = "fp8") -> HookedLM:
+        """Hold the blocks' projections in 8 bits from here on ("fp8": e4m3 with a scale per 128 x 128
+        block); they are frozen.  Under tensor parallelism shard first."""
+        if kind != "fp8":
+            raise ValueError(f"quantize_weights: kind must be 'fp8', got {kind!r}")
+        from saelens_b200.models.lm.fp8 import quantize_lm_fp8
+
+        quantize_lm_fp8(self)
+        self.cfg.weight_quantization = kind
+        return self
+
     @property
     def W_U(self) -> torch.Tensor:
         return self.embed.weight if self.unembed is None else self.unembed.weight
@@ -553,10 +674,24 @@ class HookedLM(HookedRootModule):
         return self.embed.weight.device
 
     # ---------------------------------------------------------------- forward
-    def _rotary(self, S: int) -> tuple[torch.Tensor, torch.Tensor] | None:
-        if self.cfg.positional != "rotary":
+    def _rotary(self, S: int) -> tuple[torch.Tensor, torch.Tensor] | RotaryFrequencies | None:
+        cfg = self.cfg
+        if cfg.positional != "rotary":
             return None
         dev = self.embed.weight.device
+        scaling = cfg.rope_scaling or {}
+        kind = scaling.get("rope_type", scaling.get("type")) or "default"
+        if kind != "default" or cfg.rotary_interleaved or cfg.rotary_dim not in (None, cfg.d_head):
+            # only a dynamic stretch depends on the length
+            key = (dev, S if kind == "dynamic" else 0)
+            if self._freq is None or self._freq[0] != key:
+                from saelens_b200.ops import rotary_frequencies
+
+                scaling = {"original_max_position_embeddings": cfg.n_ctx, **scaling} if kind == "dynamic" else scaling
+                freq, factor = rotary_frequencies(cfg.rotary_dim or cfg.d_head or 0, cfg.rotary_base, scaling or None,
+                                                  n_positions=S, device=dev)
+                self._freq = (key, RotaryFrequencies(freq, factor, cfg.rotary_interleaved))
+            return self._freq[1]
         if self._rot is None or self._rot[0].shape[0] < S or self._rot[0].device != dev:
             self._rot = rotary_tables(max(S, self.cfg.n_ctx), self.cfg.d_head or 0, self.cfg.rotary_base, dev)
         return self._rot[0][:S], self._rot[1][:S]
@@ -612,13 +747,24 @@ class HookedLM(HookedRootModule):
             x, S, start = residual, residual.shape[1], start_at_layer
         rot = self._rotary(S)
         end = self.cfg.n_layers if stop_at_layer is None else min(stop_at_layer, self.cfg.n_layers)
-        for blk in self.blocks[start:end]:
-            x = blk(x, rot)
-        if stop_at_layer is not None and stop_at_layer < self.cfg.n_layers:
+        stops = stop_at_layer is not None and stop_at_layer < self.cfg.n_layers
+        normed = None
+        for i in range(start, end):
+            blk, then = self.blocks[i], None
+            # the norm that reads this block's stream next, when nothing can change the stream before it
+            if not _unwatched(blk):
+                pass
+            elif i + 1 < end:
+                if _unwatched(self.blocks[i + 1]) and _plain(self.blocks[i + 1].hook_resid_pre):
+                    then = self.blocks[i + 1].ln1
+            elif not stops and return_type is not None:
+                then = self.ln_final
+            x, normed = blk(x, rot, normed, then) if then is not None else (blk(x, rot, normed), None)
+        if stops:
             return x
         if return_type is None:
             return None
-        x = self.ln_final(x)
+        x = self.ln_final(x) if normed is None else self.ln_final.hook_normalized(normed)
         if return_type == "residual":
             return x
         logits = _tied_unembed(x, self.W_U) if self.unembed is None else self.unembed(x)
