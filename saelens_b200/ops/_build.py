@@ -44,6 +44,7 @@ SOURCES = [
     "rotary.cu",
     "block_norm.cu",
     "fp8.cu",
+    "block_ops.cpp",
 ]
 
 NVCC_FLAGS = [

@@ -9,6 +9,8 @@
 #include <tuple>
 #include <vector>
 
+#include "block_ops.h"
+
 namespace sb {
 void gemm_tn_bf16(const torch::Tensor& A, const torch::Tensor& B, const c10::optional<torch::Tensor>& bias,
                   const c10::optional<torch::Tensor>& scale, bool relu,
@@ -131,31 +133,16 @@ void p2p_wait_targets(const torch::Tensor& counters, const torch::Tensor& target
 void p2p_signal(const std::vector<int64_t>& peer_bases, int64_t rank, int64_t off, int64_t index,
                 int64_t rank_mask, int64_t value);
 torch::Tensor rmsnorm(const torch::Tensor& x, const torch::Tensor& w, double eps, bool one_plus);
-void residual_norm_fwd(const torch::Tensor& x, const torch::Tensor& branch, const torch::Tensor& w,
-                       const c10::optional<torch::Tensor>& b, const c10::optional<torch::Tensor>& post_w,
-                       const c10::optional<torch::Tensor>& post_b, const c10::optional<torch::Tensor>& gate,
-                       int64_t gate_div, double eps, double post_eps, double scale, bool layer, bool one_plus,
-                       bool round_branch, const torch::Tensor& stream, const torch::Tensor& normed,
-                       const c10::optional<torch::Tensor>& stats);
-bool residual_norm_bwd_fits(int64_t D, int64_t sums);
-void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::optional<torch::Tensor>& d_normed,
-                       const torch::Tensor& stream, const torch::Tensor& branch, const torch::Tensor& w,
-                       const c10::optional<torch::Tensor>& post_w, const c10::optional<torch::Tensor>& post_b,
-                       const c10::optional<torch::Tensor>& gate, int64_t gate_div, int64_t gate_mode, double scale,
-                       bool layer, bool one_plus, const torch::Tensor& stats, const torch::Tensor& dx,
-                       const c10::optional<torch::Tensor>& dbranch, const c10::optional<torch::Tensor>& dw,
-                       const c10::optional<torch::Tensor>& db, const c10::optional<torch::Tensor>& dpost_w,
-                       const c10::optional<torch::Tensor>& dpost_b, const c10::optional<torch::Tensor>& dgate);
-void rotary_fwd(const torch::Tensor& q, const c10::optional<torch::Tensor>& k, const torch::Tensor& freq,
-                const c10::optional<torch::Tensor>& positions, int64_t pos0, bool interleaved, bool inverse,
-                double factor, const torch::Tensor& q_out, const c10::optional<torch::Tensor>& k_out);
-std::tuple<torch::Tensor, torch::Tensor> quantize_fp8(const torch::Tensor& x, int64_t block_rows);
-void linear_fp8(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& scale,
-                const c10::optional<torch::Tensor>& bias, bool transposed, const torch::Tensor& out,
-                const torch::Tensor& status);
-void gemm_fp8(const torch::Tensor& a, const torch::Tensor& a_scale, const torch::Tensor& weight,
-              const torch::Tensor& scale, const c10::optional<torch::Tensor>& bias, const torch::Tensor& out,
-              const torch::Tensor& status);
+torch::Tensor linear_fp8(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& scale,
+                         const c10::optional<torch::Tensor>& bias, const torch::Tensor& status, bool read_status);
+std::tuple<torch::Tensor, torch::Tensor> residual_norm(
+    const torch::Tensor& x, const torch::Tensor& branch, const torch::Tensor& w, const c10::optional<torch::Tensor>& b,
+    bool layer, double eps, bool one_plus, const c10::optional<torch::Tensor>& post_w,
+    const c10::optional<torch::Tensor>& post_b, double post_eps, const c10::optional<torch::Tensor>& gate, double scale,
+    bool round_branch);
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> rotary(
+    const torch::Tensor& q, const c10::optional<torch::Tensor>& k, const torch::Tensor& freq,
+    const c10::optional<torch::Tensor>& positions, int64_t offset, bool interleaved, double factor, bool inplace);
 void rope_(const torch::Tensor& x, const torch::Tensor& cos, const torch::Tensor& sin, int64_t pos0);
 torch::Tensor gated_act(const torch::Tensor& gate, const torch::Tensor& up, int64_t kind);
 torch::Tensor layernorm(const torch::Tensor& x, const torch::Tensor& w, const c10::optional<torch::Tensor>& b,
@@ -273,12 +260,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("cmax"), py::arg("status"), py::arg("ticket"), py::arg("max_ctas") = 0, py::arg("tmax") = py::none());
   m.def("rmsnorm", &sb::rmsnorm);
   m.def("rope_", &sb::rope_);
-  m.def("residual_norm_fwd", &sb::residual_norm_fwd);
-  m.def("residual_norm_bwd", &sb::residual_norm_bwd);
-  m.def("residual_norm_bwd_fits", &sb::residual_norm_bwd_fits);
-  m.def("rotary_fwd", &sb::rotary_fwd);
-  m.def("quantize_fp8", &sb::quantize_fp8);
   m.def("linear_fp8", &sb::linear_fp8);
+  m.def("residual_norm", &sb::residual_norm);
+  m.def("rotary", &sb::rotary);
+  m.def("quantize_fp8", &sb::quantize_fp8);
   m.def("gemm_fp8", &sb::gemm_fp8);
   m.def("gated_act", &sb::gated_act);
   m.def("layernorm", &sb::layernorm);

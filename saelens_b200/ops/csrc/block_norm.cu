@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "block_ops.h"
 #include "check.h"
 #include "vec.cuh"
 

@@ -33,3 +33,6 @@ inline std::string check_msg(const A&... a) {
 }  // namespace sb
 
 #define SB_CHECK(cond, ...) TORCH_CHECK((cond), ::sb::detail::check_msg(__VA_ARGS__).c_str())
+
+// The same for what a caller passed: a Python ValueError.
+#define SB_VALUE(cond, ...) TORCH_CHECK_VALUE((cond), ::sb::detail::check_msg(__VA_ARGS__).c_str())

@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <tuple>
 
+#include "block_ops.h"
 #include "check.h"
 #include "common.cuh"
 #include "tmap.h"
@@ -630,19 +631,20 @@ __global__ void __launch_bounds__(320, 1)
       const float* xs = a.xs + row;
       const float* ws = a.ws + (col0 / BLK) * a.ws_f;
       const bool in = row < a.M && col0 < a.F;
-      auto scale = [&](int rb) { return in && rb < RB ? xs[rb * a.ldxs] * ws[rb * a.ws_r] : 0.f; };
+      // two blocks ahead, and multiplied only where they are used, so that nothing waits for them
+      auto load = [&](int rb) { return in && rb < RB ? make_float2(xs[rb * a.ldxs], ws[rb * a.ws_r]) : make_float2(0.f, 0.f); };
       uint64_t acc[COLS / 2];
 #pragma unroll
       for (int c = 0; c < COLS / 2; ++c) acc[c] = 0ull;
-      float s0 = scale(0), s1 = scale(1);
+      float2 s0 = load(0), s1 = load(1);
       for (int rb = 0; rb < RB; ++rb, ++it) {
-        const float s2 = scale(rb + 2);
+        const float2 s2 = load(rb + 2);
         const int c = it & 1;
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&tfull[c], (it >> 1) & 1, abort_flag, a.status, kTimeoutEpilogue));
         if (!ok) break;  // the warp leaves as one
         tc_fence_after();
         const uint32_t at = tmem + (uint32_t(q * 32) << 16) + c * BN + half * COLS;
-        const uint64_t sc = both(s0);
+        const uint64_t sc = both(s0.x * s0.y);
 #pragma unroll
         for (int h = 0; h < COLS / 32; ++h) {
           uint32_t r[32];
@@ -934,9 +936,9 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_fp8(const torch::Tensor& x, in
 
 // out = quantised x times the weight (transposed: the product over the weight's rows, the gradient
 // of x), plus bias.  x [rows, R] bf16, fp16 or fp32; weight e4m3 [N, K], scales [N / 128, K / 128].
-void linear_fp8(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& scale,
-                const c10::optional<torch::Tensor>& bias, bool transposed, const torch::Tensor& out,
-                const torch::Tensor& status) {
+void fp8_product(const torch::Tensor& x, const torch::Tensor& weight, const torch::Tensor& scale,
+                 const c10::optional<torch::Tensor>& bias, bool transposed, const torch::Tensor& out,
+                 const torch::Tensor& status) {
   fp8::check_rows(x, "linear_fp8");
   const fp8::Weight w = fp8::weight_of(weight, scale, transposed);
   SB_CHECK(x.device() == weight.device() && x.size(1) == w.R, "linear_fp8: x must be [rows, ", w.R, "] on the weight's device");

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 
+#include "block_ops.h"
 #include "check.h"
 #include "vec.cuh"
 

@@ -8,8 +8,8 @@ reference's producer engine (the engine arguments of sae_lens/vllm_model.py:548-
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
+from saelens_b200.ops._build import load
 from saelens_b200.ops.status import StatusWord
 
 __all__ = ["quantize_fp8", "gemm_fp8", "linear_fp8"]
@@ -20,12 +20,6 @@ _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 def _blocks(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK
-
-
-def _rows_contiguous(t: torch.Tensor) -> torch.Tensor:
-    """t [..., K] as [rows, K] with contiguous rows (a view where the layout allows it)."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
@@ -44,10 +38,8 @@ def quantize_fp8(x: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, to
         raise ValueError(f"quantize_fp8: block_rows must be 1 or {BLOCK}, got {block_rows}")
     if not x.is_cuda:
         raise ValueError("quantize_fp8: x must be on a CUDA device")
-    from saelens_b200.ops import native
-
     x = x.detach()
-    return native().quantize_fp8(x if x.stride(1) == 1 else x.contiguous(), block_rows)
+    return load().quantize_fp8(x if x.stride(1) == 1 else x.contiguous(), block_rows)
 
 
 def _check_weight(name: str, width: int, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None,
@@ -93,40 +85,11 @@ def gemm_fp8(
         if out_dtype not in _FLOATS:
             raise ValueError(f"gemm_fp8: out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
         out = torch.empty(M, b.shape[0], dtype=out_dtype, device=a.device)
-    from saelens_b200.ops import native
-
     st = status or StatusWord(a.device)
-    native().gemm_fp8(a, a_scale, b, b_scale, bias, out, st.tensor)
+    load().gemm_fp8(a, a_scale, b, b_scale, bias, out, st.tensor)
     if status is None:
         st.check("gemm_fp8")
     return out
-
-
-def _product(x: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None, transposed: bool,
-             status: StatusWord | None) -> torch.Tensor:
-    from saelens_b200.ops import native
-
-    x2 = _rows_contiguous(x)
-    out = torch.empty(x2.shape[0], weight.shape[1 if transposed else 0], dtype=x.dtype, device=x.device)
-    st = status or StatusWord(x.device)
-    native().linear_fp8(x2, weight, scale, bias, transposed, out, st.tensor)
-    if status is None:
-        st.check("linear_fp8")
-    return out.view(*x.shape[:-1], out.shape[1])
-
-
-class _LinearFp8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, scale, bias, status):
-        ctx.save_for_backward(weight, scale)
-        ctx.status = status
-        return _product(x, weight, scale, bias, False, status)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        weight, scale = ctx.saved_tensors
-        return _product(dy, weight, scale, None, True, ctx.status), None, None, None, None
 
 
 def linear_fp8(
@@ -145,12 +108,12 @@ def linear_fp8(
     same way (the quantisation of x counts as the identity).  Without `status` every call reads its
     own status word, which waits for the device; a program passes one word and checks it when it
     waits anyway (and has to under CUDA graph capture)."""
+    if x.is_cuda and status is not None:  # checked where it is launched
+        return load().linear_fp8(x, weight, scale, bias, status.tensor, False)
     if x.dim() < 1 or x.dtype not in _FLOATS or x.shape[-1] < 1:
         raise ValueError(f"linear_fp8: x must be bf16, fp16 or fp32 [..., width], got {x.dtype} {tuple(x.shape)}")
     _check_weight("linear_fp8", x.shape[-1], weight, scale, bias, x.device)
-    if torch.is_grad_enabled():
-        if scale.requires_grad or (bias is not None and bias.requires_grad) or weight.requires_grad:
-            raise ValueError("linear_fp8: the weight, its scales and the bias are frozen; only x has a gradient")
-        if x.requires_grad:
-            return _LinearFp8.apply(x, weight, scale, bias, status)
-    return _product(x, weight, scale, bias, False, status)
+    st = StatusWord(x.device)
+    y = load().linear_fp8(x, weight, scale, bias, st.tensor, True)
+    st.check("linear_fp8")
+    return y

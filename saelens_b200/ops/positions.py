@@ -7,6 +7,8 @@ from typing import Any
 
 import torch
 
+from saelens_b200.ops._build import load
+
 __all__ = ["rotary", "rotary_frequencies"]
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -66,46 +68,6 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict[str, Any] 
     return (freq * (1 - ramp) + freq / factor * ramp).to(device), attention
 
 
-def _turn(q, k, freq, positions, offset, interleaved, inverse, factor, q_out, k_out):
-    from saelens_b200.ops import native
-
-    native().rotary_fwd(q, k, freq, positions, offset, interleaved, inverse, factor, q_out, k_out)
-
-
-def _last_contiguous(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, freq, positions, offset, interleaved, inverse, factor):
-        ctx.save_for_backward(freq, positions)
-        ctx.args = (offset, interleaved, inverse, factor)
-        ctx.set_materialize_grads(False)
-        q = _last_contiguous(q)
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = None
-        if k is not None:
-            k = _last_contiguous(k)
-            k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _turn(q, k, freq, positions, offset, interleaved, inverse, factor, q_out, k_out)
-        return q_out if k is None else (q_out, k_out)
-
-    @staticmethod
-    def backward(ctx, dq, dk=None):
-        # the transposed rotation, differentiable in its turn
-        freq, positions = ctx.saved_tensors
-        offset, interleaved, inverse, factor = ctx.args
-        rest = (freq, positions, offset, interleaved, not inverse, factor)
-        if dq is not None and dk is not None:
-            dq, dk = _Rotary.apply(dq, dk, *rest)
-        elif dq is not None:
-            dq = _Rotary.apply(dq, None, *rest)
-        elif dk is not None:
-            dk = _Rotary.apply(dk, None, *rest)
-        return (dq, dk) + (None,) * 6
-
-
 def rotary(
     q: torch.Tensor,
     k: torch.Tensor | None,
@@ -125,6 +87,9 @@ def rotary(
     (`rotary_frequencies`).  `positions` int64 or int32, [B, S] or what broadcasts to it, any value;
     without it token s is at offset + s.  Returns new tensors, or with `inplace` q and k themselves
     (not under autograd).  Differentiable in q and k."""
+    if q.is_cuda:  # checked where it is launched
+        out = load().rotary(q, k, freq, positions, offset, interleaved, factor, inplace)
+        return out if k is not None else out[0]
     if q.dim() != 4 or q.dtype not in _FLOATS:
         raise ValueError(f"rotary: q must be bf16, fp16 or fp32 [B, S, H, d], got {q.dtype} {tuple(q.shape)}")
     B, S, _, d = q.shape
@@ -137,31 +102,6 @@ def rotary(
             raise ValueError(f"rotary: positions must be int64 or int32 [B, S], got {positions.dtype} {tuple(positions.shape)}")
         if offset:
             raise ValueError("rotary: either positions or an offset")
-        try:
-            positions = positions.expand(B, S)
-        except RuntimeError:
-            raise ValueError(f"rotary: positions {tuple(positions.shape)} do not broadcast to {(B, S)}") from None
-    if not q.is_cuda or freq.device != q.device or (positions is not None and positions.device != q.device):
-        raise ValueError("rotary: all tensors must be on one CUDA device")
-    freq = freq.contiguous()
-    grad = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
-    args = (freq, positions, int(offset), bool(interleaved), False, float(factor))
-    if inplace:
-        if grad:
-            raise ValueError("rotary: not in place where gradients are wanted")
-        for t in (q, k):
-            if t is not None and (any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())) or (d > 1 and t.stride(3) != 1)):
-                raise ValueError("rotary: in place needs contiguous channels and no value twice")
-        _turn(q, k, *args, q, k)
-        return q if k is None else (q, k)
-    if grad:
-        return _Rotary.apply(q, k, *args)
-    q = _last_contiguous(q)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k is None:
-        _turn(q, None, *args, q_out, None)
-        return q_out
-    k = _last_contiguous(k)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _turn(q, k, *args, q_out, k_out)
-    return q_out, k_out
+        if any(n not in (1, want) for n, want in zip(reversed(positions.shape), (S, B))):
+            raise ValueError(f"rotary: positions {tuple(positions.shape)} do not broadcast to {(B, S)}")
+    raise ValueError("rotary: all tensors must be on one CUDA device")

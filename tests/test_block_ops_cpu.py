@@ -71,18 +71,6 @@ def test_residual_norm_refuses(change, match):
         ops.residual_norm(**{**norm_args(), **change})
 
 
-def test_gates_by_their_rows():
-    from saelens_b200.ops.norms import _gate_rows
-
-    shape = torch.Size((2, 3, 5, 8))
-    for own, rows, div, mode in (((), 1, 30, 1), ((1, 1, 1), 1, 30, 1), ((2, 1, 1), 2, 15, 2), ((2, 3, 1), 6, 5, 2),
-                                 ((2, 3, 5), 30, 1, 3)):
-        g, d, m = _gate_rows(torch.zeros(*own, 8), shape)
-        assert (g.shape, d, m) == ((rows, 8), div, mode)
-    assert _gate_rows(torch.zeros(4, 1, 8), torch.Size((4, 1, 8)))[1:] == (1, 3)
-    assert _gate_rows(torch.zeros(8), torch.Size((8,)))[1:] == (1, 1)
-
-
 @pytest.mark.parametrize("change,match", [
     ({"q": torch.zeros(2, 3, 16)}, "q must be"),
     ({"q": torch.zeros(2, 3, 4, 16, dtype=torch.float64)}, "q must be"),

@@ -230,24 +230,37 @@ def test_outputs_beyond_32_bit_offsets():
         check_product(y[rows], *product_ref(xq, xs, wq, ws, None), k)
 
 
-def test_refusals_of_the_kernels():
-    from saelens_b200.ops import StatusWord, native
+def test_refusals_on_the_device():
+    from saelens_b200 import ops
 
-    st = StatusWord("cuda").tensor
+    st = ops.StatusWord("cuda")
     wq, ws = weight(256, 256)
     x = torch.randn(4, 256, device="cuda").to(BF)
+    xq, xs = ops.quantize_fp8(x, 1)
     out = torch.empty(4, 256, device="cuda", dtype=BF)
-    nat = native()
-    for bad in (lambda: nat.linear_fp8(x[:, :100], wq, ws, None, False, out, st),
-                lambda: nat.linear_fp8(x, wq[:, 1:], ws, None, False, out, st),
-                lambda: nat.linear_fp8(x, wq, ws[:1], None, False, out, st),
-                lambda: nat.linear_fp8(x, wq, ws, None, False, out[:3], st),
-                lambda: nat.linear_fp8(x, wq, ws, ws[0], False, out, st),
-                lambda: nat.linear_fp8(x.cpu(), wq, ws, None, False, out, st),
-                lambda: nat.linear_fp8(x, wq, ws.cpu(), None, False, out, st),
-                lambda: nat.linear_fp8(x, x, ws, None, False, out, st),
-                lambda: nat.gemm_fp8(wq[:4], ws[:1].expand(4, -1), wq, ws, None, out, st),
-                lambda: nat.gemm_fp8(wq[:4], torch.ones(2, 4, device="cuda").T, wq, ws, None, out, st),
-                lambda: nat.quantize_fp8(x, 2)):
-        with pytest.raises(RuntimeError):
+    for bad in (lambda: ops.linear_fp8(x[:, :100], wq, ws, status=st),
+                lambda: ops.linear_fp8(x.double(), wq, ws, status=st),
+                lambda: ops.linear_fp8(x[:, 1:], wq[:, 1:], ws, status=st),
+                lambda: ops.linear_fp8(x, wq, ws[:1], status=st),
+                lambda: ops.linear_fp8(x, wq, ws.double(), status=st),
+                lambda: ops.linear_fp8(x, wq, ws, ws[0], status=st),
+                lambda: ops.linear_fp8(x, wq, ws, torch.zeros(256, device="cuda", dtype=BF), status=st),
+                lambda: ops.linear_fp8(x, wq, ws.cpu(), status=st),
+                lambda: ops.linear_fp8(x, wq.cpu(), ws, status=st),
+                lambda: ops.linear_fp8(x, x, ws, status=st),
+                lambda: ops.linear_fp8(x, wq, ws, torch.zeros(256, device="cuda", requires_grad=True), status=st),
+                lambda: ops.linear_fp8(x, wq, ws.clone().requires_grad_(), status=st),
+                lambda: ops.gemm_fp8(xq, xs, wq, ws, out=out[:3]),
+                lambda: ops.gemm_fp8(xq, xs, wq, ws, out=out.double()),
+                lambda: ops.gemm_fp8(xq, xs, wq, ws, out=out.t()),
+                lambda: ops.gemm_fp8(xq, xs.contiguous(), wq, ws),
+                lambda: ops.gemm_fp8(xq, torch.ones(2, 4, device="cuda").T, wq, ws),
+                lambda: ops.quantize_fp8(x, 2)):
+        with pytest.raises((RuntimeError, ValueError)):
             bad()
+    # twice differentiable it is not
+    x = x.requires_grad_()
+    y = ops.linear_fp8(x, wq, ws, status=st)
+    g = torch.ones_like(y).requires_grad_()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y, x, g, create_graph=True)

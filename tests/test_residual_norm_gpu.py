@@ -297,3 +297,24 @@ def test_rows_beyond_32_bit_offsets():
     for part in (slice(0, 2), slice(rows - 2, rows)):
         a, b = ops.residual_norm(x[part].clone(), x[part].clone(), w, eps=EPS)
         assert torch.equal(s[part], a) and torch.equal(y[part], b)
+
+
+def test_refusals_on_the_device():
+    from saelens_b200 import ops
+
+    x, w = torch.randn(2, 3, 64, device="cuda"), torch.randn(64, device="cuda")
+    for kw in ({"branch": x[:1]}, {"branch": x.to(BF)}, {"weight": w[:63]}, {"weight": w.cpu()}, {"bias": w}, {"kind": "batch"},
+               {"kind": "layer", "post_bias": w}, {"gate": x[:1]}, {"gate": x[..., :1]}, {"gate": x.cpu()}, {"x": x.double()},
+               {"x": torch.zeros(2, 16392, device="cuda"), "branch": torch.zeros(2, 16392, device="cuda"), "weight": torch.zeros(16392, device="cuda")},
+               {"x": torch.zeros(2, 8193, device="cuda"), "branch": torch.zeros(2, 8193, device="cuda"), "weight": torch.zeros(8193, device="cuda")}):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.residual_norm(**{"x": x, "branch": x, "weight": w, **kw})
+    d = 16384  # four column sums of which do not fit, three do
+    a = torch.randn(2, d, device="cuda").requires_grad_()
+    v = [torch.randn(d, device="cuda").requires_grad_() for _ in range(4)]
+    with pytest.raises(ValueError, match="do not fit"):
+        ops.residual_norm(a, a.detach(), v[0], v[1], kind="layer", post_weight=v[2], post_bias=v[3])
+    s, y = ops.residual_norm(a, a.detach(), v[0], v[1], kind="layer", post_weight=v[2])
+    g = torch.ones_like(y).requires_grad_()
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(y, a, g, create_graph=True)

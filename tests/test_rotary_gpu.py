@@ -5,8 +5,6 @@ Tolerance: the fraction of a turn is rounded to fp32 (2^-25 of at most half a tu
 16 2^-24 (|a| + |b|) factor covers them; the output is rounded once, by eps / 2.  Positions enter in
 64 bits: p * freq / 2 pi is off by 2^-51 of itself, and so is the reference's angle."""
 
-import math
-
 import pytest
 import torch
 
@@ -172,20 +170,20 @@ def test_beyond_32_bit_offsets():
         check(out[:, a:b], q[:, a:b], torch.arange(a, b, device="cuda")[None], f, False)
 
 
-def test_refusals_of_the_kernel():
-    from saelens_b200.ops import native
+def test_refusals_on_the_device():
+    from saelens_b200 import ops
 
     q = torch.randn(2, 3, 4, 64, device="cuda")
     f = freqs(64)
-    nat = native()
-    for bad in (lambda: nat.rotary_fwd(q, None, f.float(), None, 0, False, False, 1.0, q, None),
-                lambda: nat.rotary_fwd(q, None, torch.cat([f, f]), None, 0, False, False, 1.0, q, None),
-                lambda: nat.rotary_fwd(q, q[:1], f, None, 0, False, False, 1.0, q, q[:1]),
-                lambda: nat.rotary_fwd(q, q, f, None, 0, False, False, 1.0, q, None),
-                lambda: nat.rotary_fwd(q, None, f, torch.zeros(2, 2, dtype=torch.int64, device="cuda"), 0, False, False, 1.0, q, None),
-                lambda: nat.rotary_fwd(q, None, f, torch.zeros(2, 3, device="cuda"), 0, False, False, 1.0, q, None),
-                lambda: nat.rotary_fwd(q.cpu(), None, f, None, 0, False, False, 1.0, q, None),
-                lambda: nat.rotary_fwd(q, None, f, None, 0, False, False, 1.0, q.half(), None)):
-        with pytest.raises(RuntimeError):
+    for bad in (lambda: ops.rotary(q, None, f.float()), lambda: ops.rotary(q, None, torch.cat([f, f])), lambda: ops.rotary(q, None, f.cpu()),
+                lambda: ops.rotary(q.double(), None, f), lambda: ops.rotary(q[0], None, f), lambda: ops.rotary(q, q[:1], f),
+                lambda: ops.rotary(q, q.to(BF), f), lambda: ops.rotary(q, q.cpu(), f),
+                lambda: ops.rotary(q, None, f, positions=torch.zeros(2, 2, dtype=torch.int64, device="cuda")),
+                lambda: ops.rotary(q, None, f, positions=torch.zeros(2, 3, device="cuda")),
+                lambda: ops.rotary(q, None, f, positions=torch.zeros(2, 3, dtype=torch.int64)),
+                lambda: ops.rotary(q, None, f, positions=torch.zeros(2, 3, dtype=torch.int64, device="cuda"), offset=2),
+                lambda: ops.rotary(q[:1].expand(2, -1, -1, -1), None, f, inplace=True),
+                lambda: ops.rotary(q.clone().requires_grad_(), None, f, inplace=True),
+                lambda: ops.rotary(torch.randn(1, 2, 2, 128, device="cuda")[..., ::2], None, f, inplace=True)):
+        with pytest.raises(ValueError):
             bad()
-    assert math.isfinite(q.sum().item())
