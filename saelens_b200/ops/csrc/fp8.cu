@@ -42,14 +42,30 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 
 __device__ __forceinline__ float quotient(float v, float most) { return v * 0.4375f / most * 1024.f; }
 
+// e4m3 of 448 v / most.  A product with 448 / most is off by less than 8 units in the last place of
+// fp32, so it rounds to the same e4m3 value unless that many from a border (the 20 bits behind the 3
+// that e4m3 keeps are near 0x80000) or below 2^-6, where e4m3's steps are no longer relative; only
+// then the quotient is formed.  Dividing every value made the quantisation issue-bound: 41 us for
+// 8192 x 4096 values, whose bytes take 15.
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float most) {
+  const float by = MAXV / most;
+  float t[8];
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    t[j] = v[j] * by;
+    const uint32_t b = abs_bits(t[j]);
+    near = near || ((b - (0x80000u - 8u)) & 0xfffffu) <= 16u || (b < 0x3c800000u && b != 0u);
+  }
+  if (near) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = quotient(v[j], most);
+  }
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(quotient(v[4 * h], most), quotient(v[4 * h + 1], most)),
-                                                 __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-        make_float2(quotient(v[4 * h + 2], most), quotient(v[4 * h + 3], most)), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * h], t[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * h + 2], t[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
     w[h] = lo | (hi << 16);
   }
   return make_uint2(w[0], w[1]);
@@ -168,6 +184,15 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, ui
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// Over a pair of blocks, issued by its first one.
+__device__ __forceinline__ void umma_e4m3_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -175,25 +200,43 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
-// 16-byte aligned bulk copy global -> this CTA's shared memory, counted on `bar`.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Arrival on a barrier of either block of a pair, ordered within this block: the accumulator has been
+// read (tcgen05.wait::ld), and no other memory is handed over.  A cluster-wide release waits for
+// every access under way and took twice the time of the products.
+__device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
 
+// mbar_wait_bounded with its clock off the path: a wait is on the way of every block of 128 here, and
+// reading the clock after the first failed try made a block's hand-over several times as long.  The
+// limit is the same.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int code) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_bounded(bar, parity, abort, status, code);
+}
+
 struct Prod {
   const void* x;        // fused quantisation: the rows themselves
   int64_t ldx;
-  const float* xs;      // [blocks of the reduction][ldxs], a row's scale at its index
-  int64_t ldxs;
   const float* ws;      // scale of (feature block, reduction block) at fb * ws_f + rb * ws_r
   int64_t ws_f, ws_r;
   const float* bias;    // [features] or nullptr
@@ -219,27 +262,30 @@ template <int NT>
 struct Few {
   static constexpr int W_BYTES = BLK * BLK, X_BYTES = NT * BLK, STAGE = W_BYTES + X_BYTES;
   static constexpr int STAGES = NT <= 16 ? 6 : NT <= 32 ? 5 : 4;
-  static constexpr int RING = STAGES + 2;  // scales outlive their tile by the two accumulators
-  static constexpr int TMEM = 2 * NT < 32 ? 32 : 2 * NT;
-  static constexpr int SMEM = STAGES * STAGE + RING * NT * 4 + 1024 + 512;
+  // accumulators: the products run so many blocks ahead of the sums
+  static constexpr int ACC = NT <= 16 ? 8 : 4;
+  static constexpr int RING = STAGES + ACC;  // scales outlive their tile by the accumulators
+  static constexpr int SLOT = NT < 32 ? 32 : NT;  // floats of a slot: a TMA copy starts on 128 bytes of shared memory
+  static constexpr int TMEM = ACC * NT;
+  static constexpr int SMEM = STAGES * STAGE + RING * SLOT * 4 + 1024 + 512;
 };
 
 template <int NT, bool FUSED, bool ALIGNED, bool W_MN, class TX, class TO>
 __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
     few_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                    const __grid_constant__ Prod a) {
+                    const __grid_constant__ CUtensorMap tmS, const __grid_constant__ Prod a) {
   using C = Few<NT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = smem + C::STAGES * C::W_BYTES;
-  float* sS = reinterpret_cast<float*>(sX + C::STAGES * C::X_BYTES);  // [RING][NT]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sS + C::RING * NT);
+  float* sS = reinterpret_cast<float*>(sX + C::STAGES * C::X_BYTES);  // [RING][SLOT]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sS + C::RING * C::SLOT);
   uint64_t* empty = full + C::STAGES;
   uint64_t* sfull = empty + C::STAGES;
   uint64_t* tfull = sfull + C::RING;
-  uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint64_t* tempty = tfull + C::ACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + C::ACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -247,27 +293,42 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
   const int RB = (a.R + BLK - 1) / BLK;
   const int rb0 = int(int64_t(split) * RB / a.splits), n = int(int64_t(split + 1) * RB / a.splits) - rb0;
 
+  auto load_w = [&](int j) {
+    const int s = j % C::STAGES, r = (rb0 + j) * BLK;
+    mbar_arrive_expect_tx(&full[s], FUSED ? C::W_BYTES : C::STAGE + NT * 4);
+    if (W_MN) tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], fb * BLK, r);
+    else tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], r, fb * BLK);
+  };
+  // the weight depends on no kernel before: its first tiles are on their way before anything else
+  const int first = min(n, C::STAGES);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], FUSED ? 1 + a.M : 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < C::RING; ++s) mbar_init(&sfull[s], FUSED ? a.M : 1);
-    for (int s = 0; s < 2; ++s) {
+    if (FUSED)
+      for (int s = 0; s < C::RING; ++s) mbar_init(&sfull[s], a.M);
+    for (int s = 0; s < C::ACC; ++s) {
       mbar_init(&tfull[s], 1);
       mbar_init(&tempty[s], 4);
     }
     *abort_flag = 0;
     fence_mbar_init();
+    for (int j = 0; j < first; ++j) load_w(j);
+    if (!FUSED) tma_prefetch_desc(&tmX);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, C::TMEM);
     tmem_relinquish();
   }
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmW);
-    if (!FUSED) tma_prefetch_desc(&tmX);
-  }
+  // items of the quantising half-warps: item i is 128 values of row i % M of reduction block i / M
+  const int hw = (threadIdx.x - 192) >> 4, l = threadIdx.x & 15;
+  float v[8];
+  auto load_item = [&](int i) {
+    const int j = i < n * a.M ? i / a.M : 0, m = i < n * a.M ? i - j * a.M : 0;
+    load8<TX, ALIGNED>(static_cast<const TX*>(a.x) + m * a.ldx, int64_t(rb0 + j) * BLK + l * 8, i < n * a.M ? a.R : 0, v);
+  };
+  if (FUSED && warp >= 6) load_item(hw);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -280,38 +341,23 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
 
   if (warp == 0) {
     if (elect_one()) {
-      auto load_w = [&](int j) {
-        const int s = j % C::STAGES, r = (rb0 + j) * BLK;
-        if (W_MN) tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], fb * BLK, r);
-        else tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], r, fb * BLK);
-      };
       auto load_x = [&](int j) {
-        const int s = j % C::STAGES, g = j % C::RING;
+        const int s = j % C::STAGES;
         tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], (rb0 + j) * BLK, 0);
-        mbar_arrive_expect_tx(&sfull[g], NT * 4);
-        bulk_load(sS + g * NT, a.xs + int64_t(rb0 + j) * a.ldxs, NT * 4, &sfull[g]);
+        tma_load_2d(sS + (j % C::RING) * C::SLOT, &tmS, &full[s], 0, rb0 + j);
       };
-      const uint32_t tx = FUSED ? C::W_BYTES : C::STAGE;
-      // the weight does not depend on the kernel that quantises x: its first tiles are on their way
-      // before that kernel ends
-      const int ahead = min(n, C::STAGES);
-      for (int j = 0; j < ahead; ++j) {
-        mbar_arrive_expect_tx(&full[j], tx);
-        load_w(j);
-      }
-      int j = ahead;
       bool ok = true;
       if (!FUSED) {
         grid_dependency_wait();
-        for (int i = 0; i < ahead; ++i) load_x(i);
+        for (int i = 0; i < first; ++i) load_x(i);
       }
+      int j = first;
       for (; j < n; ++j) {
         const int s = j % C::STAGES;
-        if (!mbar_wait_bounded(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
+        if (!wait_bar(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
           ok = false;
           break;
         }
-        mbar_arrive_expect_tx(&full[s], tx);
         load_w(j);
         if (!FUSED) load_x(j);
       }
@@ -319,7 +365,6 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
         for (int i = max(0, j - C::STAGES); i < j; ++i) {
           volatile int dummy = 0;
           mbar_wait_bounded(&full[i % C::STAGES], (i / C::STAGES) & 1, &dummy, nullptr, 0);
-          if (!FUSED) mbar_wait_bounded(&sfull[i % C::RING], (i / C::RING) & 1, &dummy, nullptr, 0);
         }
       }
     }
@@ -328,9 +373,9 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
     if (elect_one()) {
       constexpr uint32_t idesc = make_idesc(128, NT, W_MN, false);
       for (int j = 0; j < n; ++j) {
-        const int s = j % C::STAGES, t = j & 1;
-        if (!mbar_wait_bounded(&tempty[t], ((j >> 1) & 1) ^ 1, abort_flag, a.status, kTimeoutMmaTmemEmpty)) break;
-        if (!mbar_wait_bounded(&full[s], (j / C::STAGES) & 1, abort_flag, a.status, kTimeoutMmaFull)) break;
+        const int s = j % C::STAGES, t = j % C::ACC;
+        if (!wait_bar(&tempty[t], ((j / C::ACC) & 1) ^ 1, abort_flag, a.status, kTimeoutMmaTmemEmpty)) break;
+        if (!wait_bar(&full[s], (j / C::STAGES) & 1, abort_flag, a.status, kTimeoutMmaFull)) break;
         tc_fence_after();
         const uint32_t w = smem_u32(sW + s * C::W_BYTES), x = smem_u32(sX + s * C::X_BYTES);
 #pragma unroll
@@ -347,16 +392,18 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
     for (int j = 0; j < n; ++j) {
       if ((j & 31) == 0 && j + lane < n) wv = a.ws[fb * a.ws_f + (rb0 + j + lane) * a.ws_r];
       const float ws = __shfl_sync(0xffffffffu, wv, j & 31);
-      const int t = j & 1, g = j % C::RING;
-      bool ok = mbar_wait_bounded(&sfull[g], (j / C::RING) & 1, abort_flag, a.status, kTimeoutEpilogue);
-      ok = ok && mbar_wait_bounded(&tfull[t], (j >> 1) & 1, abort_flag, a.status, kTimeoutEpilogue);
+      const int t = j % C::ACC, g = j % C::RING;
+      bool ok = true;
+      // the products waited for the scales that came with their tile; those written here have their own barrier
+      if (FUSED) ok = wait_bar(&sfull[g], (j / C::RING) & 1, abort_flag, a.status, kTimeoutEpilogue);
+      ok = ok && wait_bar(&tfull[t], (j / C::ACC) & 1, abort_flag, a.status, kTimeoutEpilogue);
       if (!__all_sync(0xffffffffu, ok)) break;  // the warp leaves as one
       tc_fence_after();
       uint32_t r[NT];
 #pragma unroll
       for (int c = 0; c < NT; c += 16) tmem_ld_x16(tmem + (uint32_t(q * 32) << 16) + t * NT + c, r + c);
       tmem_ld_wait();
-      const float4* xs = reinterpret_cast<const float4*>(sS + g * NT);
+      const float4* xs = reinterpret_cast<const float4*>(sS + g * C::SLOT);
 #pragma unroll
       for (int c = 0; c < NT; c += 4) {
         const float4 v = xs[c / 4];
@@ -371,8 +418,6 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
     }
     __syncwarp();
   } else if (FUSED) {
-    // item i: 128 values of row i % M of the block's reduction block i / M
-    const int hw = (threadIdx.x - 192) >> 4, l = threadIdx.x & 15;
     const uint32_t mask = 0xffffu << (lane & 16);
     const int items = n * a.M;
     // every half-warp takes part in the warp's shuffles, with or without an item of its own
@@ -380,17 +425,16 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
       const int i = i0 + (hw & 1);
       const bool have = i < items;
       const int j = have ? i / a.M : 0, m = have ? i - j * a.M : 0;
-      float v[8];
-      load8<TX, ALIGNED>(static_cast<const TX*>(a.x) + m * a.ldx, int64_t(rb0 + j) * BLK + l * 8, have ? a.R : 0, v);
       const float most = half_warp_most(v);
       const uint2 w = quantize8(v, most);
+      load_item(i + 8);  // the next one's values arrive meanwhile
       const int s = j % C::STAGES, g = j % C::RING;
       bool ok = true;
-      if (have) ok = mbar_wait_bounded(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer);
+      if (have) ok = wait_bar(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer);
       if (have && ok) {
         // row m of the stage's tile in the 128-byte swizzle: 16-byte granule l / 2 at (l / 2) ^ (m % 8)
         *reinterpret_cast<uint2*>(sX + s * C::X_BYTES + m * BLK + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8) = w;
-        if (l == 0) sS[g * NT + m] = most / MAXV;
+        if (l == 0) sS[g * C::SLOT + m] = most / MAXV;
         fence_proxy_async_smem();
         __syncwarp(mask);
         if (l == 0) {
@@ -438,18 +482,27 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
 }
 
 // ---- many rows ------------------------------------------------------------------------------
-// Persistent, one block an SM: tiles of 128 rows by BN features, each block of 128 of the reduction in
-// one of two TMEM accumulators.
-//   warps 0..7  scaled sums in registers: a row a thread, BN / 2 features (warps 0-3 the first half)
-//   warp 8      TMA;  warp 9  tcgen05.mma
-template <int BN>
+// Persistent; PAIR: two SMs (a cluster of 2) share a 256 x 256 tile by one cta_group::2 product, each
+// staging half of either operand, else one SM has a 128 x 128 tile.  A stage's bytes pass shared
+// memory twice, written by TMA and read by the tensor core: 64 KB for 512 cycles of products in a
+// pair, 96 KB on one SM with a 128 x 256 tile, which that bounds.  Every block of 128 of the
+// reduction goes to one of two TMEM accumulators.
+//   warps 0..7   scaled sums in registers: a row a thread, half of the tile's features (warps 0-3 the first)
+//   warp 8       TMA;  warp 9  tcgen05.mma (in the pair's first block);  warps 10, 11 only give up registers
+template <bool PAIR, int BN_>
 struct Many {
-  static constexpr int X_BYTES = 128 * BLK, W_BYTES = BN * BLK, STAGE = X_BYTES + W_BYTES;
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
-  static constexpr int OUT = 32 * 128;  // one warp's staging tile: 32 rows of 128 bytes
-  static constexpr int SMEM = STAGES * STAGE + 8 * OUT + 1024 + 256;
+  static constexpr int BM = PAIR ? 256 : 128, BN = BN_, W_ROWS = PAIR ? BN / 2 : BN;
+  static constexpr int X_BYTES = 128 * BLK, W_BYTES = W_ROWS * BLK, STAGE = X_BYTES + W_BYTES;  // of one block
+  static constexpr int STAGES = W_ROWS == 256 ? 3 : 5;
+  static constexpr int RING = STAGES + 2;  // row scales outlive their tile by the two accumulators
+  static constexpr int OUT = 32 * 128;     // one warp's staging tile: 32 rows of 128 bytes
+  static constexpr int SMEM = STAGES * STAGE + 8 * OUT + RING * 512 + 1024 + 256;
   static constexpr int GROUP = 4096 / BN;  // feature tiles walked together (L2 reuse)
+  static constexpr int COLS = BN / 2;      // features of a thread
+  // registers of a thread: the launch gives 168, the summing warps take what the others give up
+  static constexpr int REGS_SUM = 224, REGS_REST = 56;
 };
+constexpr int MANY_THREADS = 384;
 
 __device__ __forceinline__ void walk(int t, int num_m, int num_f, int group, int& mt, int& ft) {
   const int g = t / (num_m * group), first = g * group;
@@ -457,21 +510,6 @@ __device__ __forceinline__ void walk(int t, int num_m, int num_f, int group, int
   const int r = t - g * num_m * group;
   mt = r / size;
   ft = first + r % size;
-}
-
-// acc (two fp32) += t (two fp32) * s
-__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s2) {
-  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(lo), "r"(hi), "l"(s2));
-}
-__device__ __forceinline__ uint64_t both(float s) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(v) : "f"(s));
-  return v;
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
 }
 
 // A warp stores 128 bytes of each of its 32 rows (lane: row `lane`, values v, from column c0 of the
@@ -509,25 +547,28 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, const float* v, TO* o
   __syncwarp();
 }
 
-template <int BN, bool W_MN, class TO>
-__global__ void __launch_bounds__(320, 1)
+template <bool PAIR, int BN, bool W_MN, class TO>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
     many_rows_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                     const __grid_constant__ Prod a) {
-  using C = Many<BN>;
+                     const __grid_constant__ CUtensorMap tmS, const __grid_constant__ Prod a) {
+  using C = Many<PAIR, BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
   uint8_t* sW = smem + C::STAGES * C::X_BYTES;
   uint8_t* sOut = smem + C::STAGES * C::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 8 * C::OUT);
-  uint64_t* empty = full + C::STAGES;
-  uint64_t* tfull = empty + C::STAGES;
-  uint64_t* tempty = tfull + 2;
+  float* sS = reinterpret_cast<float*>(sOut + 8 * C::OUT);       // [RING][128] scales of the block's rows
+  uint64_t* full = reinterpret_cast<uint64_t*>(sS + C::RING * 128);  // in the first block: both blocks' loads
+  uint64_t* empty = full + C::STAGES;                            // in each block
+  uint64_t* tfull = empty + C::STAGES;                           // in each block
+  uint64_t* tempty = tfull + 2;                                  // in the first block: both blocks' warps
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_m = (a.M + 127) / 128, num_f = (a.F + BN - 1) / BN, tiles = num_m * num_f;
+  const int cta = PAIR ? int(cluster_ctarank()) : 0;
+  const int first_tile = PAIR ? blockIdx.x >> 1 : blockIdx.x, tile_step = PAIR ? gridDim.x >> 1 : gridDim.x;
+  const int num_m = (a.M + C::BM - 1) / C::BM, num_f = (a.F + C::BN - 1) / C::BN, tiles = num_m * num_f;
   const int RB = (a.R + BLK - 1) / BLK;
 
   if (threadIdx.x == 0) {
@@ -537,14 +578,19 @@ __global__ void __launch_bounds__(320, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&tfull[s], 1);
-      mbar_init(&tempty[s], 8);
+      mbar_init(&tempty[s], PAIR ? 16 : 8);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   if (warp == 9) {
-    tmem_alloc(tmem_slot, 2 * BN);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(tmem_slot, 2 * C::BN);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 2 * C::BN);
+      tmem_relinquish();
+    }
   }
   if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&tmX);
@@ -552,141 +598,176 @@ __global__ void __launch_bounds__(320, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();  // both blocks' barriers stand before any remote arrival
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
 
-  if (warp == 8) {
-    if (elect_one()) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        int mt, ft;
-        walk(t, num_m, num_f, C::GROUP, mt, ft);
-        for (int rb = 0; rb < RB; ++rb, ++it) {
-          const int s = it % C::STAGES;
-          if (!mbar_wait_bounded(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&full[s], C::STAGE);
-          tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], rb * BLK, mt * 128);
-          if (W_MN) {
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_REST));
+    if (warp == 8) {
+      if (elect_one()) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = first_tile; t < tiles && ok; t += tile_step) {
+          int mt, ft;
+          walk(t, num_m, num_f, C::GROUP, mt, ft);
+          const int row = mt * C::BM + cta * 128, col = ft * C::BN + cta * C::W_ROWS;
+          for (int rb = 0; rb < RB; ++rb, ++it) {
+            const int s = it % C::STAGES;
+            if (!wait_bar(&empty[s], ((it / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
+              ok = false;
+              break;
+            }
+            float* ss = sS + (it % C::RING) * 128;
+            if (PAIR) {
+              const uint32_t fb = mapa_shared(smem_u32(&full[s]), 0);
+              if (cta == 0) mbar_arrive_expect_tx(&full[s], 2 * (C::STAGE + 512));
+              tma_load_2d_pair(sX + s * C::X_BYTES, &tmX, fb, rb * BLK, row);
+              tma_load_2d_pair(ss, &tmS, fb, row, rb);
+              if (W_MN) tma_load_2d_pair(sW + s * C::W_BYTES, &tmW, fb, col, rb * BLK);
+              else tma_load_2d_pair(sW + s * C::W_BYTES, &tmW, fb, rb * BLK, col);
+            } else {
+              mbar_arrive_expect_tx(&full[s], C::STAGE + 512);
+              tma_load_2d(sX + s * C::X_BYTES, &tmX, &full[s], rb * BLK, row);
+              tma_load_2d(ss, &tmS, &full[s], row, rb);
+              if (W_MN) {
 #pragma unroll
-            for (int c = 0; c < BN / 128; ++c)
-              tma_load_2d(sW + s * C::W_BYTES + c * 16384, &tmW, &full[s], ft * BN + c * 128, rb * BLK);
-          } else {
-            tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], rb * BLK, ft * BN);
+                for (int c = 0; c < C::W_ROWS / 128; ++c)
+                  tma_load_2d(sW + s * C::W_BYTES + c * 16384, &tmW, &full[s], col + c * 128, rb * BLK);
+              } else tma_load_2d(sW + s * C::W_BYTES, &tmW, &full[s], rb * BLK, col);
+            }
+          }
+        }
+        if (!ok && cta == 0) {  // the copies in flight land before the block leaves
+          const uint32_t first = it > C::STAGES ? it - C::STAGES : 0;
+          for (uint32_t j = first; j < it; ++j) {
+            volatile int dummy = 0;
+            mbar_wait_bounded(&full[j % C::STAGES], (j / C::STAGES) & 1, &dummy, nullptr, 0);
           }
         }
       }
-      if (!ok) {
-        const uint32_t first = it > C::STAGES ? it - C::STAGES : 0;
-        for (uint32_t j = first; j < it; ++j) {
-          volatile int dummy = 0;
-          mbar_wait_bounded(&full[j % C::STAGES], (j / C::STAGES) & 1, &dummy, nullptr, 0);
-        }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    if (elect_one()) {
-      constexpr uint32_t idesc = make_idesc(128, BN, false, W_MN);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        for (int rb = 0; rb < RB; ++rb, ++it) {
-          const int s = it % C::STAGES, c = it & 1;
-          if (!mbar_wait_bounded(&tempty[c], ((it >> 1) & 1) ^ 1, abort_flag, a.status, kTimeoutMmaTmemEmpty) ||
-              !mbar_wait_bounded(&full[s], (it / C::STAGES) & 1, abort_flag, a.status, kTimeoutMmaFull)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t x = smem_u32(sX + s * C::X_BYTES), w = smem_u32(sW + s * C::W_BYTES);
+      __syncwarp();
+    } else if (warp == 9) {
+      if (cta == 0 && elect_one()) {
+        constexpr uint32_t idesc = make_idesc(C::BM, C::BN, false, W_MN);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = first_tile; t < tiles && ok; t += tile_step) {
+          for (int rb = 0; rb < RB; ++rb, ++it) {
+            const int s = it % C::STAGES, c = it & 1;
+            // the stage is there long before; the accumulator is what the products wait for
+            if (!wait_bar(&full[s], (it / C::STAGES) & 1, abort_flag, a.status, kTimeoutMmaFull) ||
+                !wait_bar(&tempty[c], ((it >> 1) & 1) ^ 1, abort_flag, a.status, kTimeoutMmaTmemEmpty)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t x = smem_u32(sX + s * C::X_BYTES), w = smem_u32(sW + s * C::W_BYTES);
 #pragma unroll
-          for (int k = 0; k < BLK / 32; ++k)
-            umma_e4m3(tmem + c * BN, make_sdesc_sw128_kmajor(x + k * 32),
-                      W_MN ? make_sdesc_sw128_mnmajor(w + k * 4096, 16384) : make_sdesc_sw128_kmajor(w + k * 32), idesc,
-                      k > 0);
-          umma_commit(&empty[s]);
-          umma_commit(&tfull[c]);
+            for (int k = 0; k < BLK / 32; ++k) {
+              const uint64_t xd = make_sdesc_sw128_kmajor(x + k * 32);
+              const uint64_t wd = W_MN ? make_sdesc_sw128_mnmajor(w + k * 4096, 16384) : make_sdesc_sw128_kmajor(w + k * 32);
+              if (PAIR) umma_e4m3_pair(tmem + c * C::BN, xd, wd, idesc, k > 0);
+              else umma_e4m3(tmem + c * C::BN, xd, wd, idesc, k > 0);
+            }
+            if (PAIR) {
+              const uint32_t e = smem_u32(&empty[s]), f = smem_u32(&tfull[c]);
+              umma_commit_pair(f);
+              umma_commit_pair(mapa_shared(f, 1));
+              umma_commit_pair(e);
+              umma_commit_pair(mapa_shared(e, 1));
+            } else {
+              umma_commit(&tfull[c]);
+              umma_commit(&empty[s]);
+            }
+          }
         }
       }
+      __syncwarp();
     }
-    __syncwarp();
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SUM));
     const int q = warp & 3, half = warp >> 2;
-    constexpr int COLS = BN / 2;
+    constexpr int COLS = C::COLS, CHUNKS = COLS / 32;
     uint8_t* stage = sOut + warp * C::OUT;
     const bool wide = (a.ldo * int64_t(sizeof(TO))) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
+    const uint32_t lead_empty = PAIR ? mapa_shared(smem_u32(tempty), 0) : 0u;
+    const uint32_t lanes = tmem + (uint32_t(q * 32) << 16) + half * COLS;
+    const float* my_scale = sS + q * 32 + lane;
     uint32_t it = 0;
+    int g = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+    for (int t = first_tile; t < tiles && ok; t += tile_step) {
       int mt, ft;
       walk(t, num_m, num_f, C::GROUP, mt, ft);
-      const int row0 = mt * 128 + q * 32, row = row0 + lane;
-      const int col0 = ft * BN + half * COLS;
-      // past the last row or feature block the sums are zeros times a scale of 0
-      const float* xs = a.xs + row;
+      const int row0 = mt * C::BM + cta * 128 + q * 32;
+      const int col0 = ft * C::BN + half * COLS;
       const float* ws = a.ws + (col0 / BLK) * a.ws_f;
-      const bool in = row < a.M && col0 < a.F;
-      // two blocks ahead, and multiplied only where they are used, so that nothing waits for them
-      auto load = [&](int rb) { return in && rb < RB ? make_float2(xs[rb * a.ldxs], ws[rb * a.ws_r]) : make_float2(0.f, 0.f); };
-      uint64_t acc[COLS / 2];
+      float wv = 0.f;  // lane l: the weight's scale of block (rb & ~31) + l
+      float acc[COLS];
 #pragma unroll
-      for (int c = 0; c < COLS / 2; ++c) acc[c] = 0ull;
-      float2 s0 = load(0), s1 = load(1);
+      for (int c = 0; c < COLS; ++c) acc[c] = 0.f;
+      // A block's turn is bounded by what this warp does in a row, so nothing in it waits: a chunk of 32
+      // columns is read while the one before it is added, and the next block's first chunk while
+      // this block's last one is, where that block's products are done by then (`ahead`).
+      uint32_t r[2][32];
+      bool ahead = false;
       for (int rb = 0; rb < RB; ++rb, ++it) {
-        const float2 s2 = load(rb + 2);
+        if ((rb & 31) == 0) wv = rb + lane < RB && col0 < a.F ? ws[(rb + lane) * a.ws_r] : 0.f;
         const int c = it & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait_bounded(&tfull[c], (it >> 1) & 1, abort_flag, a.status, kTimeoutEpilogue));
-        if (!ok) break;  // the warp leaves as one
-        tc_fence_after();
-        const uint32_t at = tmem + (uint32_t(q * 32) << 16) + c * BN + half * COLS;
-        const uint64_t sc = both(s0.x * s0.y);
+        const uint32_t at = lanes + c * C::BN;
+        if (!ahead) {
+          ok = __all_sync(0xffffffffu, wait_bar(&tfull[c], (it >> 1) & 1, abort_flag, a.status, kTimeoutEpilogue));
+          if (!ok) break;  // the warp leaves as one
+          tc_fence_after();
+          tmem_ld_32x32b_x32(at, r[0]);
+        }
+        const float sc = my_scale[g * 128] * __shfl_sync(0xffffffffu, wv, rb & 31);
+        g = g + 1 == C::RING ? 0 : g + 1;
 #pragma unroll
-        for (int h = 0; h < COLS / 32; ++h) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(at + h * 32, r);
+        for (int h = 0; h < CHUNKS; ++h) {
           tmem_ld_wait();
-          if (h == COLS / 32 - 1) {  // read out: the accumulator is free
+          if (h + 1 < CHUNKS) {
+            tmem_ld_32x32b_x32(at + (h + 1) * 32, r[(h + 1) & 1]);
+          } else {  // read out: the accumulator is free
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tempty[c]);
+            if (lane == 0) {
+              if (PAIR) mbar_arrive_pair(lead_empty + c * 8);
+              else mbar_arrive(&tempty[c]);
+            }
+            ahead = rb + 1 < RB && __all_sync(0xffffffffu, mbar_test(&tfull[c ^ 1], ((it + 1) >> 1) & 1));
+            if (ahead) {
+              tc_fence_after();
+              tmem_ld_32x32b_x32(lanes + (c ^ 1) * C::BN, r[0]);
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i) fma2(acc[h * 16 + i], r[2 * i], r[2 * i + 1], sc);
+          for (int i = 0; i < 32; ++i) acc[h * 32 + i] += __uint_as_float(r[h & 1][i]) * sc;
         }
-        s0 = s1;
-        s1 = s2;
       }
       if (!ok) break;
       constexpr int CH = 128 / int(sizeof(TO));  // columns of a staged store
 #pragma unroll
       for (int c = 0; c < COLS / CH; ++c) {
-        float v[CH];
-#pragma unroll
-        for (int i = 0; i < CH / 2; ++i) {
-          const float2 p = halves(acc[c * (CH / 2) + i]);
-          v[2 * i] = p.x;
-          v[2 * i + 1] = p.y;
-        }
         if (a.bias) {
 #pragma unroll
           for (int i = 0; i < CH; ++i)
-            if (col0 + c * CH + i < a.F) v[i] += __ldg(a.bias + col0 + c * CH + i);
+            if (col0 + c * CH + i < a.F) acc[c * CH + i] += __ldg(a.bias + col0 + c * CH + i);
         }
-        store_rows<TO>(stage, v, static_cast<TO*>(a.out), a.ldo, row0, a.M, col0 + c * CH, a.F, lane, wide);
+        store_rows<TO>(stage, acc + c * CH, static_cast<TO*>(a.out), a.ldo, row0, a.M, col0 + c * CH, a.F, lane, wide);
       }
     }
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();  // no block leaves while its pair may still touch its memory
   if (warp == 9) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    if (PAIR) tmem_dealloc_pair(tmem, 2 * C::BN);
+    else tmem_dealloc(tmem, 2 * C::BN);
   }
 }
 
@@ -773,6 +854,10 @@ static Weight weight_of(const torch::Tensor& w, const torch::Tensor& s, bool tra
   return r;
 }
 
+// Tensor maps are made by the driver, which wants a current context: a thread that has called nothing
+// of the runtime yet (autograd's, for one) has none.
+static void bind_context(const torch::Tensor& t) { C10_CUDA_CHECK(cudaSetDevice(t.device().index())); }
+
 static CUtensorMap weight_map(const Weight& w, int box_features) {
   // box: 128 along the stored row by 128 (or the tile's features) rows
   const int64_t rows = w.mn ? w.R : w.F, cols = w.mn ? w.F : w.R;
@@ -782,7 +867,7 @@ static CUtensorMap weight_map(const Weight& w, int box_features) {
 
 template <class K>
 static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st,
-                   const CUtensorMap& tW, const CUtensorMap& tX, const Prod& a) {
+                   const CUtensorMap& tW, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a) {
   C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -803,7 +888,7 @@ static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool d
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tW, tX, a));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tW, tX, tS, a));
 }
 
 constexpr int FEW = 64;         // rows up to which the few-rows kernel runs
@@ -816,13 +901,13 @@ static int splits_for(int64_t feature_tiles, int64_t reduction_blocks, int sms) 
 }
 
 template <int NT, bool FUSED, class TX, class TO>
-static void few_rows(const Weight& w, const CUtensorMap& tX, Prod a, bool x_aligned, cudaStream_t st) {
+static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, Prod a, bool x_aligned, cudaStream_t st) {
   const int64_t tiles = (w.F + BLK - 1) / BLK;
   a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
   const dim3 grid{unsigned(tiles * a.splits)};
   const CUtensorMap tW = weight_map(w, BLK);
   const int threads = FUSED ? 320 : 192, smem = Few<NT>::SMEM;
-  auto go = [&](auto kern) { launch(kern, grid, threads, smem, a.splits, a.dependent, st, tW, tX, a); };
+  auto go = [&](auto kern) { launch(kern, grid, threads, smem, a.splits, a.dependent, st, tW, tX, tS, a); };
   if constexpr (FUSED) {
     if (!x_aligned) {
       if (w.mn) go(few_rows_kernel<NT, true, false, true, TX, TO>);
@@ -834,31 +919,34 @@ static void few_rows(const Weight& w, const CUtensorMap& tX, Prod a, bool x_alig
   else go(few_rows_kernel<NT, FUSED, true, false, TX, TO>);
 }
 
-template <int BN, class TO>
-static void many_rows(const Weight& w, const CUtensorMap& tX, const Prod& a, cudaStream_t st) {
-  const int64_t tiles = ((a.M + 127) / 128) * ((w.F + BN - 1) / BN);
-  SB_CHECK(tiles < (1ll << 31), "fp8 product: too many tiles");
+template <bool PAIR, int BN, class TO>
+static void many_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a, cudaStream_t st) {
+  using C = Many<PAIR, BN>;
+  const int64_t tiles = ((a.M + C::BM - 1) / C::BM) * ((w.F + C::BN - 1) / C::BN);
+  SB_CHECK(tiles < (1ll << 30), "fp8 product: too many tiles");
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const dim3 grid{unsigned(std::min<int64_t>(tiles, sms))};
-  const CUtensorMap tW = weight_map(w, BN);
-  if (w.mn) launch(many_rows_kernel<BN, true, TO>, grid, 320, Many<BN>::SMEM, 1, a.dependent, st, tW, tX, a);
-  else launch(many_rows_kernel<BN, false, TO>, grid, 320, Many<BN>::SMEM, 1, a.dependent, st, tW, tX, a);
+  const dim3 grid{unsigned(PAIR ? 2 * std::min<int64_t>(tiles, sms / 2) : std::min<int64_t>(tiles, sms))};
+  const CUtensorMap tW = weight_map(w, C::W_ROWS);
+  const int cluster = PAIR ? 2 : 1;
+  if (w.mn) launch(many_rows_kernel<PAIR, BN, true, TO>, grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
+  else launch(many_rows_kernel<PAIR, BN, false, TO>, grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
 }
 
-// Quantised rows (uint8 [M, R] with row stride ldq, scales [blocks][lds]) times the weight.
+// Quantised rows (uint8 [M, R] with row stride ldq) and their scales ([blocks][lds]) times the weight.
 template <class TO>
-static void product(const uint8_t* q, int64_t ldq, const Weight& w, const Prod& a, cudaStream_t st) {
+static void product(const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, const Weight& w, const Prod& a, cudaStream_t st) {
   const int box = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= FEW ? 64 : 128;
   const CUtensorMap tX = make_tmap_2d(q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, w.R, ldq, box, BLK, CU_TENSOR_MAP_SWIZZLE_128B);
-  if (a.M <= 16) few_rows<16, false, float, TO>(w, tX, a, true, st);
-  else if (a.M <= 32) few_rows<32, false, float, TO>(w, tX, a, true, st);
-  else if (a.M <= FEW) few_rows<64, false, float, TO>(w, tX, a, true, st);
+  const CUtensorMap tS = make_tmap_2d(scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (w.R + BLK - 1) / BLK, a.M, lds * 4, 1, box,
+                                      CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (a.M <= 16) few_rows<16, false, float, TO>(w, tX, tS, a, true, st);
+  else if (a.M <= 32) few_rows<32, false, float, TO>(w, tX, tS, a, true, st);
+  else if (a.M <= FEW) few_rows<64, false, float, TO>(w, tX, tS, a, true, st);
   else {
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-    const int64_t m = (a.M + 127) / 128;
-    const int64_t wide_tiles = m * ((w.F + 255) / 256);
-    if (wide_tiles >= sms) many_rows<256, TO>(w, tX, a, st);
-    else many_rows<128, TO>(w, tX, a, st);
+    const int64_t pairs = ((a.M + 255) / 256) * ((w.F + 255) / 256);
+    if (pairs >= sms / 4) many_rows<true, 256, TO>(w, tX, tS, a, st);
+    else many_rows<false, 128, TO>(w, tX, tS, a, st);
   }
 }
 
@@ -891,17 +979,15 @@ static void linear_t(const torch::Tensor& x, const Weight& w, Prod a, cudaStream
   if (a.M <= FUSED_ROWS) {
     a.x = x.data_ptr();
     a.ldx = x.stride(0);
-    few_rows<16, true, T, T>(w, CUtensorMap{}, a, rows_aligned(x), st);
+    few_rows<16, true, T, T>(w, CUtensorMap{}, CUtensorMap{}, a, rows_aligned(x), st);
     return;
   }
-  const int64_t ldq = up(w.R, 16), lds = up(a.M, 64), RB = (w.R + BLK - 1) / BLK;
+  const int64_t ldq = up(w.R, 16), lds = up(a.M, 4), RB = (w.R + BLK - 1) / BLK;
   torch::Tensor q = torch::empty({a.M * ldq}, x.options().dtype(at::kByte));
   torch::Tensor s = torch::empty({RB * lds}, x.options().dtype(at::kFloat));
   quantize_rows(x, q.data_ptr<uint8_t>(), ldq, s.data_ptr<float>(), lds, st);
-  a.xs = s.data_ptr<float>();
-  a.ldxs = lds;
   a.dependent = 1;  // the quantisation itself began after everything before it had ended
-  product<T>(q.data_ptr<uint8_t>(), ldq, w, a, st);
+  product<T>(q.data_ptr<uint8_t>(), ldq, s.data_ptr<float>(), lds, w, a, st);
 }
 
 }  // namespace fp8
@@ -919,7 +1005,7 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_fp8(const torch::Tensor& x, in
   uint8_t* qp = q.data_ptr<uint8_t>();
   torch::Tensor s;
   if (block_rows == 1) {
-    const int64_t lds = fp8::up(M, 64);
+    const int64_t lds = fp8::up(M, 4);
     torch::Tensor store = torch::empty({KB, lds}, x.options().dtype(at::kFloat));
     if (M) fp8::quantize_rows(x, qp, ldq, store.data_ptr<float>(), lds, st);
     s = store.t().narrow(0, 0, M);
@@ -946,6 +1032,7 @@ void fp8_product(const torch::Tensor& x, const torch::Tensor& weight, const torc
   const fp8::Prod a = fp8::prod_of(w, x.size(0), bias, out, status, weight);
   if (a.M == 0) return;
   const at::cuda::CUDAGuard guard(x.device());
+  fp8::bind_context(x);
   auto st = at::cuda::getCurrentCUDAStream();
   if (x.scalar_type() == at::kBFloat16) fp8::linear_t<__nv_bfloat16>(x, w, a, st);
   else if (x.scalar_type() == at::kHalf) fp8::linear_t<__half>(x, w, a, st);
@@ -968,22 +1055,19 @@ void gemm_fp8(const torch::Tensor& a, const torch::Tensor& a_scale, const torch:
   SB_CHECK(a_scale.device() == a.device() && a_scale.scalar_type() == at::kFloat && a_scale.dim() == 2 &&
                a_scale.size(0) == M && a_scale.size(1) == RB && (M <= 1 || a_scale.stride(0) == 1),
            "gemm_fp8: a's scales must be fp32 [", M, ", ", RB, "] with stride 1 between rows");
-  fp8::Prod p = fp8::prod_of(w, M, bias, out, status, weight);
+  const fp8::Prod p = fp8::prod_of(w, M, bias, out, status, weight);
   if (M == 0) return;
-  // the few-rows kernel copies the scales of a whole row tile at once, in 16-byte units
-  const int64_t tile = M <= 16 ? 16 : M <= 32 ? 32 : 64;
-  p.ldxs = RB > 1 ? a_scale.stride(1) : fp8::up(M, 64);
-  const int64_t room = int64_t(a_scale.storage().nbytes() / sizeof(float)) - a_scale.storage_offset();
-  SB_CHECK(M > fp8::FEW || (p.ldxs % 4 == 0 && reinterpret_cast<uintptr_t>(a_scale.data_ptr()) % 16 == 0 &&
-                            (RB - 1) * p.ldxs + tile <= room),
-           "gemm_fp8: a's scales must be laid out as quantize_fp8 does");
-  p.xs = a_scale.data_ptr<float>();
+  const int64_t lds = RB > 1 ? a_scale.stride(1) : fp8::up(M, 4);
+  SB_CHECK(lds % 4 == 0 && lds >= M && reinterpret_cast<uintptr_t>(a_scale.data_ptr()) % 16 == 0,
+           "gemm_fp8: a's scales must be laid out as quantize_fp8 does (blocks 16-byte aligned)");
+  const float* sp = a_scale.data_ptr<float>();
   const at::cuda::CUDAGuard guard(a.device());
+  fp8::bind_context(a);
   auto st = at::cuda::getCurrentCUDAStream();
   const uint8_t* q = static_cast<const uint8_t*>(a.data_ptr());
-  if (out.scalar_type() == at::kBFloat16) fp8::product<__nv_bfloat16>(q, ldq, w, p, st);
-  else if (out.scalar_type() == at::kHalf) fp8::product<__half>(q, ldq, w, p, st);
-  else fp8::product<float>(q, ldq, w, p, st);
+  if (out.scalar_type() == at::kBFloat16) fp8::product<__nv_bfloat16>(q, ldq, sp, lds, w, p, st);
+  else if (out.scalar_type() == at::kHalf) fp8::product<__half>(q, ldq, sp, lds, w, p, st);
+  else fp8::product<float>(q, ldq, sp, lds, w, p, st);
 }
 
 }  // namespace sb

@@ -175,6 +175,24 @@ def test_shapes_streams_and_strides():
     assert torch.equal(y.reshape(-1, 300), flat)
 
 
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_from_a_new_thread(m):
+    """A thread that has called nothing of CUDA before."""
+    import threading
+
+    from saelens_b200 import ops
+
+    wq, ws = weight(300, 264)
+    x = torch.randn(m, 264, device="cuda").to(BF)
+    st = ops.StatusWord("cuda")
+    torch.cuda.synchronize()
+    got = []
+    t = threading.Thread(target=lambda: got.append(ops.linear_fp8(x, wq, ws, status=st)))
+    t.start()
+    t.join()
+    assert torch.equal(got[0], ops.linear_fp8(x, wq, ws, status=st))
+
+
 @pytest.mark.parametrize("m", [1, 16, 40, 200])
 def test_a_bad_row_stays_alone(m):
     from saelens_b200 import ops
@@ -254,7 +272,7 @@ def test_refusals_on_the_device():
                 lambda: ops.gemm_fp8(xq, xs, wq, ws, out=out.double()),
                 lambda: ops.gemm_fp8(xq, xs, wq, ws, out=out.t()),
                 lambda: ops.gemm_fp8(xq, xs.contiguous(), wq, ws),
-                lambda: ops.gemm_fp8(xq, torch.ones(2, 4, device="cuda").T, wq, ws),
+                lambda: ops.gemm_fp8(xq, torch.ones(2, 5, device="cuda")[:, :4].T, wq, ws),
                 lambda: ops.quantize_fp8(x, 2)):
         with pytest.raises((RuntimeError, ValueError)):
             bad()
