@@ -19,6 +19,7 @@
 #include <torch/types.h>
 
 #include <algorithm>
+#include <atomic>
 #include <tuple>
 
 #include "block_ops.h"
@@ -219,11 +220,11 @@ __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepco
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // mbar_wait_bounded with its clock off the path: a wait is on the way of every block of 128 here, and
 // reading the clock after the first failed try made a block's hand-over several times as long.  The
@@ -232,6 +233,29 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
   for (int i = 0; i < 64; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   return mbar_wait_bounded(bar, parity, abort, status, code);
+}
+
+__device__ __forceinline__ void st_release_cta(int* p, int v) {
+  asm volatile("st.release.cta.shared.b32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+// Wait until the count at p reaches `least`; limits as for a barrier.
+__device__ __forceinline__ bool wait_count(int* p, int least, volatile int* abort, int* status, int code) {
+  unsigned long long t0 = 0;
+  for (int i = 0;; ++i) {
+    int v;
+    asm volatile("ld.acquire.cta.shared.b32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+    if (v >= least) return true;
+    if ((i & 63) == 63) {
+      if (*abort) return false;
+      const unsigned long long now = globaltimer_ns();
+      if (!t0) t0 = now;
+      if (now - t0 > kWaitTimeoutNs) {
+        *abort = 1;
+        if (status) atomicCAS(status, 0, code);
+        return false;
+      }
+    }
+  }
 }
 
 struct Prod {
@@ -251,9 +275,11 @@ struct Prod {
 // ---- few rows -------------------------------------------------------------------------------
 // Up to NT rows.  The weight is the tensor cores' 128-row operand and the rows of x the narrow one, so
 // that no part of the tile is idle weight; the time is the weight's bytes.  A block owns 128
-// features and a part of the reduction; the blocks of a cluster hold the parts of the same features
-// and add their sums over distributed shared memory in block order.  Two blocks share an SM (half
-// its shared memory each): the grid then fills it with finer parts.
+// features and a part of the reduction; the blocks of a cluster hold the parts of the same features.
+// Column c of the sums belongs to block c % splits: every block writes its part of it there, over
+// distributed shared memory, and after one cluster barrier the owner adds the parts in block order.
+// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)  Two blocks
+// share an SM, half its shared memory each: the grid then fills it with finer parts.
 //   warp 0      weight tiles by TMA (and x tiles and scales, unless they are quantised here)
 //   warp 1      tcgen05.mma, 4 a block of 128
 //   warps 2..5  scaled sums in registers: a feature a thread, NT columns
@@ -261,13 +287,14 @@ struct Prod {
 template <int NT>
 struct Few {
   static constexpr int W_BYTES = BLK * BLK, X_BYTES = NT * BLK, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = NT <= 16 ? 6 : NT <= 32 ? 5 : 4;
+  static constexpr int STAGES = NT <= 16 ? 5 : NT <= 32 ? 4 : 3;
   // accumulators: the products run so many blocks ahead of the sums
   static constexpr int ACC = NT <= 16 ? 8 : 4;
   static constexpr int RING = STAGES + ACC;  // scales outlive their tile by the accumulators
   static constexpr int SLOT = NT < 32 ? 32 : NT;  // floats of a slot: a TMA copy starts on 128 bytes of shared memory
   static constexpr int TMEM = ACC * NT;
-  static constexpr int SMEM = STAGES * STAGE + RING * SLOT * 4 + 1024 + 512;
+  // parts of the columns that a block owns: [columns][splits][128 features], NT + splits - 1 of 512 bytes at most
+  static constexpr int SMEM = STAGES * STAGE + RING * SLOT * 4 + (NT + 8) * 512 + 1024 + 512;
 };
 
 template <int NT, bool FUSED, bool ALIGNED, bool W_MN, class TX, class TO>
@@ -280,13 +307,15 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
   uint8_t* sW = smem;
   uint8_t* sX = smem + C::STAGES * C::W_BYTES;
   float* sS = reinterpret_cast<float*>(sX + C::STAGES * C::X_BYTES);  // [RING][SLOT]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sS + C::RING * C::SLOT);
+  float* parts = sS + C::RING * C::SLOT;
+  uint64_t* full = reinterpret_cast<uint64_t*>(parts + (NT + 8) * 128);
   uint64_t* empty = full + C::STAGES;
   uint64_t* sfull = empty + C::STAGES;
   uint64_t* tfull = sfull + C::RING;
   uint64_t* tempty = tfull + C::ACC;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + C::ACC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* released = reinterpret_cast<int*>(tmem_slot + 2);  // FUSED: blocks below this have a free stage
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x % a.splits, fb = blockIdx.x / a.splits;
@@ -313,6 +342,7 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
       mbar_init(&tempty[s], 4);
     }
     *abort_flag = 0;
+    *released = first;
     fence_mbar_init();
     for (int j = 0; j < first; ++j) load_w(j);
     if (!FUSED) tma_prefetch_desc(&tmX);
@@ -329,6 +359,9 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
     load8<TX, ALIGNED>(static_cast<const TX*>(a.x) + m * a.ldx, int64_t(rb0 + j) * BLK + l * 8, i < n * a.M ? a.R : 0, v);
   };
   if (FUSED && warp >= 6) load_item(hw);
+  // the cluster's blocks have all started once this barrier is through, which is asked for only at the end
+  __syncwarp();
+  if (a.splits > 1) cluster_arrive_relaxed();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -358,6 +391,7 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
           ok = false;
           break;
         }
+        if (FUSED) st_release_cta(released, j + 1);
         load_w(j);
         if (!FUSED) load_x(j);
       }
@@ -430,7 +464,9 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
       load_item(i + 8);  // the next one's values arrive meanwhile
       const int s = j % C::STAGES, g = j % C::RING;
       bool ok = true;
-      if (have) ok = wait_bar(&empty[s], ((j / C::STAGES) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer);
+      // A half-warp skips blocks, so a stage's barrier may be several phases from the one it would wait
+      // for and its parity says nothing; the loading thread has waited for each phase and counts them.
+      if (have) ok = wait_count(released, j + 1, abort_flag, a.status, kTimeoutTmaProducer);
       if (have && ok) {
         // row m of the stage's tile in the 128-byte swizzle: 16-byte granule l / 2 at (l / 2) ^ (m % 8)
         *reinterpret_cast<uint2*>(sX + s * C::X_BYTES + m * BLK + (((l >> 1) ^ (m & 7)) << 4) + (l & 1) * 8) = w;
@@ -445,6 +481,7 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
       __syncwarp();
       if (__any_sync(0xffffffffu, !ok)) break;
     }
+    __syncwarp();
   }
 
   auto store = [&](int m, float v) {
@@ -457,21 +494,21 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
       for (int c = 0; c < NT; ++c)
         if (c < a.M) store(c, acc[c]);
   } else {
-    // every tile of the block has been multiplied: its memory holds the sums for the cluster
-    float* red = reinterpret_cast<float*>(smem);  // [NT][128]
-    if (sums)
-#pragma unroll
-      for (int c = 0; c < NT; ++c) red[c * BLK + q * 32 + lane] = acc[c];
-    cluster_sync_all();
+    cluster_wait();
     if (sums) {
-      const uint32_t mine = smem_u32(red) + uint32_t(q * 32 + lane) * 4;
+      const uint32_t mine = smem_u32(parts) + uint32_t(split * BLK + q * 32 + lane) * 4;
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+        if (c < a.M) st_cluster_f32(mapa_shared(mine + uint32_t(c / a.splits * a.splits) * BLK * 4, uint32_t(c % a.splits)), acc[c]);
+    }
+    cluster_sync_all();
+    if (sums)
       for (int c = split; c < a.M; c += a.splits) {
+        const float* p = parts + (c / a.splits * a.splits) * BLK + q * 32 + lane;
         float v = 0.f;
-        for (int p = 0; p < a.splits; ++p) v += ld_cluster_f32(mapa_shared(mine + uint32_t(c) * BLK * 4, uint32_t(p)));
+        for (int k = 0; k < a.splits; ++k) v += p[k * BLK];
         store(c, v);
       }
-    }
-    cluster_sync_all();  // no block leaves while another may read its sums
   }
   tc_fence_before();
   __syncthreads();
@@ -865,10 +902,18 @@ static CUtensorMap weight_map(const Weight& w, int box_features) {
                       CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// All of an SM's shared memory, asked for: left to itself the runtime divides it for one block, and two
+// that would fit run after one another.
+template <class K>
+static void set_shared(K kern, int smem) {
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+}
+
 template <class K>
 static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st,
                    const CUtensorMap& tW, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a) {
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  set_shared(kern, smem);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = grid;
@@ -892,22 +937,53 @@ static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool d
 }
 
 constexpr int FEW = 64;         // rows up to which the few-rows kernel runs
-constexpr int FUSED_ROWS = 16;  // rows up to which it quantises them itself
+constexpr int FUSED_ROWS = 2;  // rows up to which it quantises them itself (of 4096 -> 6144: 2 rows 12 us, apart 14.6; 4 rows 17 against 14)
 
-// Parts of the reduction: so many that two blocks for every SM are running, 8 at most.
-static int splits_for(int64_t feature_tiles, int64_t reduction_blocks, int sms) {
-  const int64_t s = (2 * sms) / feature_tiles;
-  return int(std::max<int64_t>(1, std::min<int64_t>({s, 8, reduction_blocks})));
+// How many clusters of `size` blocks run at once (asked for once for each shape of kernel and device).
+template <int NT, bool FUSED, class K>
+static int clusters_at_once(K kern, int size, int threads, int smem, int device) {
+  constexpr int DEVICES = 32;
+  static std::atomic<int> known[DEVICES][9];
+  std::atomic<int>* cell = device < DEVICES ? &known[device][size] : nullptr;
+  if (cell && cell->load()) return cell->load();
+  set_shared(kern, smem);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+  n = std::max(1, n);
+  if (cell) cell->store(n);
+  return n;
+}
+
+// Parts of the reduction: the most, up to 8, with which all clusters run at once.  A second wave of a
+// few clusters cost as much as the first (48 feature tiles in 6 parts: 12.6 us, in one wave 8).
+template <int NT, bool FUSED, class K>
+static int splits_for(K kern, int64_t feature_tiles, int64_t reduction_blocks, int threads, int smem, int device) {
+  for (int s = int(std::min<int64_t>(8, reduction_blocks)); s > 1; --s)
+    if (feature_tiles * s <= 512 && feature_tiles <= clusters_at_once<NT, FUSED>(kern, s, threads, smem, device)) return s;
+  return 1;
 }
 
 template <int NT, bool FUSED, class TX, class TO>
 static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, Prod a, bool x_aligned, cudaStream_t st) {
   const int64_t tiles = (w.F + BLK - 1) / BLK;
-  a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-  const dim3 grid{unsigned(tiles * a.splits)};
+  SB_CHECK(tiles < (1ll << 27), "fp8 product: size of the weight");
   const CUtensorMap tW = weight_map(w, BLK);
   const int threads = FUSED ? 320 : 192, smem = Few<NT>::SMEM;
-  auto go = [&](auto kern) { launch(kern, grid, threads, smem, a.splits, a.dependent, st, tW, tX, tS, a); };
+  auto go = [&](auto kern) {
+    a.splits = splits_for<NT, FUSED>(kern, tiles, (w.R + BLK - 1) / BLK, threads, smem, c10::cuda::current_device());
+    launch(kern, dim3(unsigned(tiles * a.splits)), threads, smem, a.splits, a.dependent, st, tW, tX, tS, a);
+  };
   if constexpr (FUSED) {
     if (!x_aligned) {
       if (w.mn) go(few_rows_kernel<NT, true, false, true, TX, TO>);

@@ -89,7 +89,7 @@ def test_quantize_strided_and_special_values():
     assert ops.quantize_fp8(x[:0], 1)[1].shape == (0, 2)
 
 
-SIZES = [(1, 128, 128), (1, 4096, 640), (2, 1, 1), (5, 130, 129), (16, 1024, 257), (17, 1024, 384), (24, 3584, 520),
+SIZES = [(1, 128, 128), (1, 4096, 640), (1, 28672, 20000), (2, 14336, 8192), (2, 1, 1), (4, 9000, 6150), (5, 130, 129), (16, 1024, 257), (17, 1024, 384), (24, 3584, 520),
          (32, 333, 100), (33, 2048, 1000), (64, 640, 2048), (65, 640, 2048), (127, 100, 300), (129, 1152, 130),
          (333, 5120, 1111), (1000, 2056, 2304), (2048, 512, 6200)]
 
