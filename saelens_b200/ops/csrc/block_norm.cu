@@ -17,8 +17,8 @@
 // deterministic: thread t holds the vectors t, t + threads, ..., lanes are joined by a butterfly
 // and warps in order, and a layer norm's weight and bias enter as one fused multiply-add, as in the
 // single norms of the producer, so that the results are theirs bit for bit.
-// Column sums of the backward pass are kept in shared memory by the thread that owns the column,
-// over the consecutive rows of its block; a second kernel adds the blocks' sums in block order.
+// Column sums of the backward pass are kept by the thread that owns the column, over consecutive
+// rows; a second kernel adds the blocks' sums in block order.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/types.h>
@@ -48,21 +48,6 @@ __device__ __forceinline__ float block_sum(float v, float* red, int warps) {
     if (i < warps) t += red[i];
   return t;
 }
-__device__ __forceinline__ float2 block_sum2(float2 v, float2* red, int warps) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float2 t = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int i = 0; i < WARPS; ++i)
-    if (i < warps) t.x += red[i].x, t.y += red[i].y;
-  return t;
-}
-
 struct Fwd {
   const void *x, *branch, *w, *b, *post_w, *post_b, *gate;
   int64_t ldx, ldb;    // row strides of x and branch
@@ -75,8 +60,12 @@ struct Fwd {
 };
 
 // NV vectors of VEC elements a thread; POST: there is a post-norm; LAYER: layer norms.
+// What hides the latencies of a row (loads, one to four sums, vectors from the L2 cache) is other rows
+// on the SM, so registers are held to what FWD_BLOCKS blocks leave.
+template <class T, int VEC, int NV>
+constexpr int FWD_BLOCKS = VEC * NV * int(sizeof(T)) <= 16 ? 7 : VEC * NV * int(sizeof(T)) <= 32 ? 6 : VEC * NV * int(sizeof(T)) <= 64 ? 3 : 1;
 template <class T, int VEC, int NV, bool LAYER, bool POST>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Fwd a) {
+__global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(const __grid_constant__ Fwd a) {
   __shared__ float red[4][WARPS];
   using P = vec::Pack<T, VEC>;
   const int warps = blockDim.x >> 5;
@@ -85,6 +74,7 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Fw
   const T* x = static_cast<const T*>(a.x) + row * a.ldx;
   const T* br = static_cast<const T*>(a.branch) + row * a.ldb;
   const T* gate = a.gate ? static_cast<const T*>(a.gate) + (row / a.gate_div) * a.D : nullptr;
+  const float add = a.one_plus ? 1.f : 0.f;
   P px[NV], pb[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -100,20 +90,26 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Fw
     if (LAYER) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (threadIdx.x + i * blockDim.x < nvec)
+        if (threadIdx.x + i * blockDim.x < nvec) {
+          float f[VEC];
+          pb[i].unpack(f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) s += pb[i].get(j);
+          for (int j = 0; j < VEC; ++j) s += f[j];
+        }
       mean = block_sum(s, red[0], warps) / float(a.D);
       s = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (threadIdx.x + i * blockDim.x < nvec)
+      if (threadIdx.x + i * blockDim.x < nvec) {
+        float f[VEC];
+        pb[i].unpack(f);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float c = LAYER ? pb[i].get(j) - mean : pb[i].get(j);
+          const float c = LAYER ? f[j] - mean : f[j];
           s += c * c;
         }
+      }
     inv = rsqrtf(block_sum(s, red[1], warps) / float(a.D) + a.post_eps);
     if (a.post_rstd && threadIdx.x == 0) {
       a.post_rstd[row] = inv;
@@ -121,31 +117,58 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Fw
     }
   }
   float s = 0.f;
+  // u: the branch's vector, through its norm where there is one -> the stream's vector
+  auto finish = [&](int i, int v, float (&u)[VEC]) {
+    float f[VEC];
+    px[i].unpack(f);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = __fadd_rn(f[j], u[j]);  // u is a value of its own, as a stored branch is
+    px[i].pack(f);
+    px[i].store(static_cast<T*>(a.stream) + row * a.D + VEC * v);
+    px[i].unpack(f);  // as stored
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += LAYER ? f[j] : f[j] * f[j];
+  };
+  const bool plain = !gate && a.scale == 1.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int v = threadIdx.x + i * blockDim.x;
     if (v < nvec) {
-      P w, b, g;
-      if (POST) w.load(static_cast<const T*>(a.post_w) + VEC * v);
-      if (POST && LAYER && a.post_b) b.load(static_cast<const T*>(a.post_b) + VEC * v);
-      if (gate) g.load(gate + VEC * v);
+      float u[VEC];
+      pb[i].unpack(u);
+      if (POST) {
+        P w, b;
+        float fw[VEC], fb[VEC];
+        w.load(static_cast<const T*>(a.post_w) + VEC * v);
+        w.unpack(fw);
+        if (LAYER && a.post_b) b.load(static_cast<const T*>(a.post_b) + VEC * v);
+        else b.zero();
+        b.unpack(fb);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        float u = pb[i].get(j);
-        if (POST) {
-          const float wj = a.one_plus ? 1.f + w.get(j) : w.get(j);
-          if (LAYER) u = __fmaf_rn((u - mean) * inv, wj, a.post_b ? b.get(j) : 0.f);
-          else u = u * inv * wj;
-          if (a.round_branch) u = vec::rounded<T>(u);
+        for (int j = 0; j < VEC; ++j) {
+          if (LAYER) u[j] = __fmaf_rn((u[j] - mean) * inv, fw[j] + add, fb[j]);
+          else u[j] = u[j] * inv * (fw[j] + add);
         }
-        if (gate) u *= g.get(j);
-        u *= a.scale;
-        if (a.round_branch) u = vec::rounded<T>(u);
-        px[i].set(j, px[i].get(j) + u);
-        const float r = px[i].get(j);  // as stored
-        s += LAYER ? r : r * r;
+        if (a.round_branch) {
+          b.pack(u);
+          b.unpack(u);
+        }
       }
-      px[i].store(static_cast<T*>(a.stream) + row * a.D + VEC * v);
+      if (!plain) {
+        P g;
+        float fg[VEC];
+        if (gate) {
+          g.load(gate + VEC * v);
+          g.unpack(fg);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) u[j] = (gate ? u[j] * fg[j] : u[j]) * a.scale;
+        if (a.round_branch) {
+          g.pack(u);
+          g.unpack(u);
+        }
+      }
+      finish(i, v, u);
     }
   }
   float total = block_sum(s, red[2], warps);
@@ -154,9 +177,12 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Fw
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (threadIdx.x + i * blockDim.x < nvec)
+      if (threadIdx.x + i * blockDim.x < nvec) {
+        float f[VEC];
+        px[i].unpack(f);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s += (px[i].get(j) - mean) * (px[i].get(j) - mean);
+        for (int j = 0; j < VEC; ++j) s += (f[j] - mean) * (f[j] - mean);
+      }
     total = block_sum(s, red[3], warps);
   }
   inv = rsqrtf(total / float(a.D) + a.eps);
@@ -169,14 +195,17 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const __grid_constant__ Fw
     const int v = threadIdx.x + i * blockDim.x;
     if (v < nvec) {
       P w, b;
+      float f[VEC], fw[VEC], fb[VEC];
       w.load(static_cast<const T*>(a.w) + VEC * v);
+      w.unpack(fw);
       if (LAYER && a.b) b.load(static_cast<const T*>(a.b) + VEC * v);
+      else b.zero();
+      if (LAYER) b.unpack(fb);
+      px[i].unpack(f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float wj = a.one_plus ? 1.f + w.get(j) : w.get(j);
-        const float r = px[i].get(j);
-        px[i].set(j, LAYER ? __fmaf_rn((r - mean) * inv, wj, a.b ? b.get(j) : 0.f) : r * inv * wj);
-      }
+      for (int j = 0; j < VEC; ++j)
+        f[j] = LAYER ? __fmaf_rn((f[j] - mean) * inv, fw[j] + add, fb[j]) : f[j] * inv * (fw[j] + add);
+      px[i].pack(f);
       px[i].store(static_cast<T*>(a.normed) + row * a.D + VEC * v);
     }
   }
@@ -194,33 +223,76 @@ struct Bwd {
   void *dx, *dbranch;  // dbranch may be nullptr
   void* dgate;         // token gates: [rows, D]; sequence gates: [sequences, D]; else nullptr
   float* partial;      // [blocks][slots][D]
-  float* edge;         // sequence gates: [blocks][2][D], sequences that reach over a block's rows
+  float* edge;         // sequence gates: [units][2][D], sequences that reach over a unit's rows
   int slot[kSums];     // place of each sum among the `slots` that are wanted, or -1
   int slots;
-  int64_t rows, rows_per_block;
+  int64_t rows, rows_per_unit;  // a unit: the rows of one group
+  int groups, group_threads;
   int D;
   float scale;
   int one_plus;
   int gate_mode;  // 0 none, 1 channel, 2 sequence, 3 token
 };
 
+// Sum over a group of `threads` threads of the block that meet at barrier `id`.
+__device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int tid, int threads, int id) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+  }
+  if ((tid & 31) == 0) red[tid >> 5] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+  float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i)
+    if (i < threads / 32) t.x += red[i].x, t.y += red[i].y;
+  return t;
+}
+
+// A block is `groups` groups of threads, each with rows of its own.  Where a thread has one vector
+// (rows of up to 2048 values) its column sums stay in registers and a block has several groups, so
+// that rows wait for their sums side by side and there are few blocks' sums to join; wider rows keep
+// theirs in shared memory, one group a block.  4104 fp32 rows of 768 with five sums: 39 -> 17 us.
+constexpr int GROUP_THREADS = 512;
 template <class T, int VEC, int NV, bool LAYER, bool POST>
-__global__ void __launch_bounds__(THREADS) bwd_kernel(const __grid_constant__ Bwd a) {
+__global__ void __launch_bounds__(NV == 1 ? GROUP_THREADS : THREADS) bwd_kernel(const __grid_constant__ Bwd a) {
+  constexpr bool REG = NV == 1;
   // [slots][VEC][vectors]: value j of vector v at (slot * VEC + j) * nvec + v, so that neighbouring
   // threads are in neighbouring banks
   extern __shared__ float sums[];
-  __shared__ float2 red[2][2][WARPS];
+  constexpr int GROUPS = REG ? GROUP_THREADS / 32 : 1;
+  __shared__ float2 red_all[GROUPS][2][2][WARPS];
   using P = vec::Pack<T, VEC>;
-  const int warps = blockDim.x >> 5;
+  const int threads = a.group_threads;
+  const int group = threadIdx.x / threads, tid = threadIdx.x - group * threads, bar = 1 + group;
+  auto red = red_all[group];
   const int nvec = a.D / VEC;
-  const int64_t r0 = blockIdx.x * a.rows_per_block, r1 = min(r0 + a.rows_per_block, a.rows);
+  const int64_t unit = int64_t(blockIdx.x) * a.groups + group;
+  const int64_t r0 = min(unit * a.rows_per_unit, a.rows), r1 = min(r0 + a.rows_per_unit, a.rows);
   auto sum_at = [&](int slot, int v, int j) -> float& { return sums[(slot * VEC + j) * nvec + v]; };
-  for (int v = threadIdx.x; v < nvec; v += blockDim.x)
-    for (int k = 0; k < a.slots; ++k)
+  float acc[REG ? kSums : 1][VEC];
+  if (REG) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum_at(k, v, j) = 0.f;
-  // no barrier: a thread's columns are its own
-  const bool need_branch = POST || (a.gate_mode && a.slot[kGate] >= 0) || (a.gate_mode >= 2 && a.dgate);
+    for (int k = 0; k < (REG ? kSums : 1); ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[k][j] = 0.f;
+  } else {
+    for (int v = tid; v < nvec; v += threads)
+      for (int k = 0; k < a.slots; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum_at(k, v, j) = 0.f;
+    // no barrier: a thread's columns are its own
+  }
+  auto add = [&](int kind, int v, int j, float value) {
+    if (a.slot[kind] >= 0) {
+      if constexpr (REG) acc[kind][j] += value;
+      else sum_at(a.slot[kind], v, j) += value;
+    }
+  };
+  const float one = a.one_plus ? 1.f : 0.f;
+  const bool need_gate = a.gate_mode && (a.gate_mode == 3 ? a.dgate != nullptr : a.slot[kGate] >= 0);
+  const bool need_branch = POST || need_gate;
   for (int64_t row = r0; row < r1; ++row) {
     const int par = int(row - r0) & 1;  // buffers of the block sums alternate between rows
     const T* st = static_cast<const T*>(a.stream) + row * a.D;
@@ -228,7 +300,7 @@ __global__ void __launch_bounds__(THREADS) bwd_kernel(const __grid_constant__ Bw
     P pr[NV], pn[NV], ps[NV], pb[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
+      const int v = tid + i * threads;
       if (v < nvec) {
         if (a.d_normed) {
           pn[i].load(static_cast<const T*>(a.d_normed) + row * a.ld_dn + VEC * v);
@@ -240,130 +312,184 @@ __global__ void __launch_bounds__(THREADS) bwd_kernel(const __grid_constant__ Bw
       }
     }
     const float inv = a.rstd[row], mean = LAYER ? a.mean[row] : 0.f;
+    const float pinv = POST ? a.post_rstd[row] : 1.f, pmean = POST && LAYER ? a.post_mean[row] : 0.f;
     float g[NV][VEC];  // the stream's gradient
     float2 c = make_float2(0.f, 0.f);
     if (a.d_normed) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
+        const int v = tid + i * threads;
         if (v < nvec) {
           P w;
           w.load(static_cast<const T*>(a.w) + VEC * v);
+          float fw[VEC], fn[VEC], fr[VEC];
+          w.unpack(fw);
+          pn[i].unpack(fn);
+          pr[i].unpack(fr);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const float dy = pn[i].get(j), t = (LAYER ? pr[i].get(j) - mean : pr[i].get(j)) * inv;
-            const float h = dy * (a.one_plus ? 1.f + w.get(j) : w.get(j));
+            const float t = (LAYER ? fr[j] - mean : fr[j]) * inv, h = fn[j] * (fw[j] + one);
             g[i][j] = h;
             c.x += h * t;
             if (LAYER) c.y += h;
-            if (a.slot[kW] >= 0) sum_at(a.slot[kW], v, j) += dy * t;
-            if (LAYER && a.slot[kB] >= 0) sum_at(a.slot[kB], v, j) += dy;
+            add(kW, v, j, fn[j] * t);
+            if (LAYER) add(kB, v, j, fn[j]);
           }
         }
       }
-      c = block_sum2(c, red[par][0], warps);
+      c = group_sum2(c, red[par][0], tid, threads, bar);
       c.x /= float(a.D);
       c.y /= float(a.D);
     }
-    const float pinv = POST ? a.post_rstd[row] : 1.f, pmean = POST && LAYER ? a.post_mean[row] : 0.f;
     float2 e = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int v = threadIdx.x + i * blockDim.x;
+      const int v = tid + i * threads;
       if (v < nvec) {
-        P pw, pbias, pg, dg, dxp;
-        if (POST) pw.load(static_cast<const T*>(a.post_w) + VEC * v);
-        if (POST && LAYER && a.post_b) pbias.load(static_cast<const T*>(a.post_b) + VEC * v);
-        if (gate) pg.load(gate + VEC * v);
+        P pk;
+        float dr[VEC], fw[VEC], u[VEC], bh[VEC], fg[VEC];
+        ps[i].unpack(dr);
+        if (a.d_normed) {
+          float fr[VEC];
+          pr[i].unpack(fr);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float t = (LAYER ? fr[j] - mean : fr[j]) * inv;
+            dr[j] += inv * (g[i][j] - (LAYER ? c.y : 0.f) - t * c.x);
+          }
+        }
+        pk.pack(dr);
+        pk.store(static_cast<T*>(a.dx) + row * a.D + VEC * v);
+        if (POST) {
+          pk.load(static_cast<const T*>(a.post_w) + VEC * v);
+          pk.unpack(fw);
+        }
+        if (need_branch) {
+          pb[i].unpack(bh);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (POST) bh[j] = (LAYER ? bh[j] - pmean : bh[j]) * pinv;
+        }
+        if (a.gate_mode) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) u[j] = POST ? bh[j] * (fw[j] + one) : bh[j];
+          if (POST && LAYER && a.post_b) {
+            pk.load(static_cast<const T*>(a.post_b) + VEC * v);
+            pk.unpack(fg);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) u[j] += fg[j];
+          }
+          if (need_gate) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              u[j] *= a.scale * dr[j];
+              if (a.gate_mode != 3) add(kGate, v, j, u[j]);
+            }
+            if (a.gate_mode == 3) {
+              pk.pack(u);
+              pk.store(static_cast<T*>(a.dgate) + row * a.D + VEC * v);
+            }
+          }
+          pk.load(gate + VEC * v);
+          pk.unpack(fg);
+        }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          float dr = ps[i].get(j);
-          if (a.d_normed) {
-            const float t = (LAYER ? pr[i].get(j) - mean : pr[i].get(j)) * inv;
-            dr += inv * (g[i][j] - (LAYER ? c.y : 0.f) - t * c.x);
-          }
-          dxp.set(j, dr);
-          const float wj = POST ? (a.one_plus ? 1.f + pw.get(j) : pw.get(j)) : 1.f;
-          float bh = 0.f, u = 0.f;
-          if (need_branch) {
-            bh = pb[i].get(j);
-            if (POST) bh = (LAYER ? bh - pmean : bh) * pinv;
-            u = POST ? bh * wj + (LAYER && a.post_b ? pbias.get(j) : 0.f) : bh;
-          }
-          if (a.gate_mode) {
-            const float d = a.scale * dr * u;
-            if (a.gate_mode == 3) dg.set(j, d);
-            else if (a.slot[kGate] >= 0) sum_at(a.slot[kGate], v, j) += d;
-          }
-          float du = dr * a.scale;
-          if (gate) du *= pg.get(j);
+          float du = dr[j] * a.scale;
+          if (a.gate_mode) du *= fg[j];
           if (POST) {
-            if (a.slot[kPostW] >= 0) sum_at(a.slot[kPostW], v, j) += du * bh;
-            if (LAYER && a.slot[kPostB] >= 0) sum_at(a.slot[kPostB], v, j) += du;
-            du *= wj;
-            e.x += du * bh;
+            add(kPostW, v, j, du * bh[j]);
+            if (LAYER) add(kPostB, v, j, du);
+            du *= fw[j] + one;
+            e.x += du * bh[j];
             if (LAYER) e.y += du;
           }
           g[i][j] = du;
         }
-        dxp.store(static_cast<T*>(a.dx) + row * a.D + VEC * v);
-        if (a.gate_mode == 3 && a.dgate) dg.store(static_cast<T*>(a.dgate) + row * a.D + VEC * v);
       }
     }
     if (POST) {
-      e = block_sum2(e, red[par][1], warps);
+      e = group_sum2(e, red[par][1], tid, threads, bar);
       e.x /= float(a.D);
       e.y /= float(a.D);
     }
     if (a.dbranch) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int v = threadIdx.x + i * blockDim.x;
+        const int v = tid + i * threads;
         if (v < nvec) {
           P o;
+          if (POST) {
+            float fb[VEC];
+            pb[i].unpack(fb);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            float d = g[i][j];
-            if (POST) {
-              const float bh = (LAYER ? pb[i].get(j) - pmean : pb[i].get(j)) * pinv;
-              d = pinv * (d - (LAYER ? e.y : 0.f) - bh * e.x);
+            for (int j = 0; j < VEC; ++j) {
+              const float bh = (LAYER ? fb[j] - pmean : fb[j]) * pinv;
+              g[i][j] = pinv * (g[i][j] - (LAYER ? e.y : 0.f) - bh * e.x);
             }
-            o.set(j, d);
           }
+          o.pack(g[i]);
           o.store(static_cast<T*>(a.dbranch) + row * a.D + VEC * v);
         }
       }
     }
-    // a sequence ends here or the block's rows do: its gate's sum leaves the block
+    // a sequence ends here or the unit's rows do: its gate's sum leaves the unit
     if (a.gate_mode == 2 && a.slot[kGate] >= 0) {
       const int64_t q = row / a.gate_div;
       const bool ends = (row + 1) % a.gate_div == 0;
       if (ends || row + 1 == r1) {
         const bool inside = q * a.gate_div >= r0;
-        for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+        for (int v = tid; v < nvec; v += threads) {
           vec::Pack<float, VEC> f;
           P o;
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            float& acc = sum_at(a.slot[kGate], v, j);
-            f.set(j, acc);
-            o.set(j, acc);
-            acc = 0.f;
+            float& s = REG ? acc[REG ? kGate : 0][j] : sum_at(a.slot[kGate], v, j);
+            f.set(j, s);
+            o.set(j, s);
+            s = 0.f;
           }
           if (inside && ends) o.store(static_cast<T*>(a.dgate) + q * a.D + VEC * v);
-          else f.store(a.edge + (int64_t(blockIdx.x) * 2 + (inside ? 1 : 0)) * a.D + VEC * v);
+          else f.store(a.edge + (unit * 2 + (inside ? 1 : 0)) * a.D + VEC * v);
         }
       }
     }
   }
   const int out_slots = a.gate_mode == 2 && a.slot[kGate] >= 0 ? a.slots - 1 : a.slots;  // the gate's slot is the last
-  for (int v = threadIdx.x; v < nvec; v += blockDim.x)
-    for (int k = 0; k < out_slots; ++k) {
-      vec::Pack<float, VEC> f;
+  if (REG) {
+    // the groups' sums in order of the groups, through one vector of shared memory a thread and kind
+    for (int k = 0; k < kSums; ++k) {
+      if (a.slot[k] < 0 || a.slot[k] >= out_slots) continue;  // uniform
+      __syncthreads();
+      if (tid < nvec)
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f.set(j, sum_at(k, v, j));
-      f.store(a.partial + (int64_t(blockIdx.x) * out_slots + k) * a.D + VEC * v);
+        for (int j = 0; j < VEC; ++j) {
+          float value = 0.f;
+#pragma unroll
+          for (int m = 0; m < (REG ? kSums : 1); ++m) value = m == k ? acc[m][j] : value;
+          sums[(group * VEC + j) * threads + tid] = value;
+        }
+      __syncthreads();
+      for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+        vec::Pack<float, VEC> f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float t = 0.f;
+          for (int m = 0; m < a.groups; ++m) t += sums[(m * VEC + j) * threads + v];
+          f.set(j, t);
+        }
+        f.store(a.partial + (int64_t(blockIdx.x) * out_slots + a.slot[k]) * a.D + VEC * v);
+      }
     }
+  } else {
+    for (int v = tid; v < nvec; v += threads)
+      for (int k = 0; k < out_slots; ++k) {
+        vec::Pack<float, VEC> f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f.set(j, sum_at(k, v, j));
+        f.store(a.partial + (int64_t(blockIdx.x) * out_slots + k) * a.D + VEC * v);
+      }
+  }
 }
 
 struct Join {
@@ -398,17 +524,17 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) join_kernel(const __grid_const
   }
 }
 
-// Gates of sequences that lie in several blocks' rows: the blocks' parts in order.
+// Gates of sequences that lie in several units' rows: the units' parts in order.
 template <class T>
-__global__ void __launch_bounds__(256) edge_kernel(const float* edge, T* dgate, int64_t rows_per_block, int64_t S, int D) {
+__global__ void __launch_bounds__(256) edge_kernel(const float* edge, T* dgate, int64_t rows_per_unit, int64_t S, int D) {
   const int64_t q = blockIdx.x;
-  const int64_t first = q * S / rows_per_block, last = ((q + 1) * S - 1) / rows_per_block;
-  if (first == last) return;  // written by its block
+  const int64_t first = q * S / rows_per_unit, last = ((q + 1) * S - 1) / rows_per_unit;
+  if (first == last) return;  // written by its unit
   const int col = blockIdx.y * 256 + threadIdx.x;
   if (col >= D) return;
   float s = 0.f;
   for (int64_t b = first; b <= last; ++b)
-    s += edge[(b * 2 + (q * S >= b * rows_per_block ? 1 : 0)) * D + col];
+    s += edge[(b * 2 + (q * S >= b * rows_per_unit ? 1 : 0)) * D + col];
   dgate[q * D + col] = vec::from_f<T>(s);
 }
 
@@ -448,23 +574,22 @@ static void run_fwd(const Fwd& a, int64_t rows, bool wide, bool layer, cudaStrea
 }
 
 template <class T, int VEC, int NV, bool LAYER, bool POST>
-static void launch_bwd(const Bwd& a, unsigned blocks, int threads, size_t smem, cudaStream_t stream) {
+static void launch_bwd(const Bwd& a, unsigned blocks, size_t smem, cudaStream_t stream) {
   auto kern = bwd_kernel<T, VEC, NV, LAYER, POST>;
   if (smem > 40 * 1024)
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
-  kern<<<dim3(blocks), dim3(threads), smem, stream>>>(a);
+  kern<<<dim3(blocks), dim3(a.groups * a.group_threads), smem, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 template <class T>
 static void run_bwd(const Bwd& a, unsigned blocks, bool wide, bool layer, size_t smem, cudaStream_t stream) {
-  const int threads = threads_for(a.D, wide);
   with_shape(a.D, wide, [&](auto V, auto N) {
     constexpr int VEC = decltype(V)::value, NV = decltype(N)::value;
-    if (layer && a.post_w) launch_bwd<T, VEC, NV, true, true>(a, blocks, threads, smem, stream);
-    else if (layer) launch_bwd<T, VEC, NV, true, false>(a, blocks, threads, smem, stream);
-    else if (a.post_w) launch_bwd<T, VEC, NV, false, true>(a, blocks, threads, smem, stream);
-    else launch_bwd<T, VEC, NV, false, false>(a, blocks, threads, smem, stream);
+    if (layer && a.post_w) launch_bwd<T, VEC, NV, true, true>(a, blocks, smem, stream);
+    else if (layer) launch_bwd<T, VEC, NV, true, false>(a, blocks, smem, stream);
+    else if (a.post_w) launch_bwd<T, VEC, NV, false, true>(a, blocks, smem, stream);
+    else launch_bwd<T, VEC, NV, false, false>(a, blocks, smem, stream);
   });
 }
 
@@ -606,15 +731,19 @@ void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::
       if (*t) (*t)->zero_();
     return;
   }
-  const size_t smem = size_t(D) * slots * 4;
-  SB_CHECK(smem <= bnorm::MAX_SUMS, "residual_norm: ", slots, " column sums of width ", D, " do not fit shared memory");
-  // blocks: as many as are resident at once, fewer when rows are few (each block's sums are written
-  // and read again: 8 rows a block keep that below the rows' own traffic)
+  const size_t held = size_t(D) * slots * 4;
+  SB_CHECK(held <= bnorm::MAX_SUMS, "residual_norm: ", slots, " column sums of width ", D, " do not fit shared memory");
+  // units: as many as run at once, fewer when rows are few (a block's sums are written and read again)
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(1024 / bnorm::threads_for(D, wide), (220 * 1024) / int64_t(smem + 2048)));
-  const int64_t least = slots ? 8 : 1;
-  a.rows_per_block = std::max<int64_t>((rows + sms * resident - 1) / (sms * resident), std::min<int64_t>(least, (rows + sms - 1) / sms));
-  const int64_t blocks = (rows + a.rows_per_block - 1) / a.rows_per_block;
+  const bool reg = wide && D / 8 <= bnorm::THREADS;  // the kernel's NV == 1
+  a.group_threads = bnorm::threads_for(D, wide);
+  // a group's barrier is one of the block's 16, the first of which is the whole block's
+  a.groups = reg ? std::min(15, bnorm::GROUP_THREADS / a.group_threads) : 1;
+  const size_t smem = reg ? size_t(a.groups) * a.group_threads * 8 * 4 : held;
+  const int64_t resident = reg ? 1 : std::max<int64_t>(1, std::min<int64_t>(1024 / a.group_threads, (220 * 1024) / int64_t(smem + 2048)));
+  const int64_t least = slots && !reg ? 8 : 1;
+  a.rows_per_unit = std::max<int64_t>((rows + sms * resident * a.groups - 1) / (sms * resident * a.groups), std::min<int64_t>(least, (rows + sms - 1) / sms));
+  const int64_t units = (rows + a.rows_per_unit - 1) / a.rows_per_unit, blocks = (units + a.groups - 1) / a.groups;
   torch::Tensor partial, edge;
   const auto f32 = stream.options().dtype(at::kFloat);
   if (joined) {
@@ -622,7 +751,7 @@ void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::
     a.partial = partial.data_ptr<float>();
   }
   if (seq) {
-    edge = torch::empty({blocks * 2 * D}, f32);
+    edge = torch::empty({units * 2 * D}, f32);
     a.edge = edge.data_ptr<float>();
   }
   auto ptr = [](const c10::optional<torch::Tensor>& t) -> void* { return t ? t->data_ptr() : nullptr; };
@@ -650,7 +779,7 @@ void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::
     }
     if (seq) {
       bnorm::edge_kernel<T><<<dim3(unsigned(rows / gate_div), unsigned((D + 255) / 256)), dim3(256), 0, st>>>(
-          a.edge, static_cast<T*>(dgate->data_ptr()), a.rows_per_block, gate_div, int(D));
+          a.edge, static_cast<T*>(dgate->data_ptr()), a.rows_per_unit, gate_div, int(D));
       C10_CUDA_KERNEL_LAUNCH_CHECK();
     }
   };

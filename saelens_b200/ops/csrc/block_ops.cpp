@@ -78,18 +78,24 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
 };
 
 // ------------------------------------------------------------------------------ residual_norm
+Opt gate_rows(const Opt& gate) {
+  return !gate || gate->dim() == 2 ? gate : Opt(gate->view({gate->numel() / gate->size(-1), gate->size(-1)}));
+}
+
 struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& branch,
                                const torch::Tensor& w, const Opt& b, const Opt& post_w, const Opt& post_b, const Opt& gate,
                                int64_t div, int64_t mode, double eps, double post_eps, double scale, bool layer,
                                bool one_plus, bool round_branch) {
+    // shapes change inside the node: a view for each input and output would be nodes of their own
+    const torch::Tensor x2 = rows_of(x), b2 = rows_of(branch);
     torch::Tensor stream = torch::empty(x.sizes(), x.options()), normed = torch::empty(x.sizes(), x.options());
-    torch::Tensor stats = torch::empty({4, x.size(0)}, x.options().dtype(at::kFloat));
-    residual_norm_fwd(x, branch, w, b, post_w, post_b, gate, div, eps, post_eps, scale, layer, one_plus, round_branch,
-                      stream, normed, stats);
+    torch::Tensor stats = torch::empty({4, x2.size(0)}, x.options().dtype(at::kFloat));
+    residual_norm_fwd(x2, b2, w, b, post_w, post_b, gate_rows(gate), div, eps, post_eps, scale, layer, one_plus, round_branch,
+                      rows_of(stream), rows_of(normed), stats);
     auto or_none = [](const Opt& t) { return t ? *t : torch::Tensor(); };
     // the branch is read again only where its own values enter a gradient
-    ctx->save_for_backward({stream, post_w || gate ? branch : torch::Tensor(), w, or_none(post_w), or_none(post_b), or_none(gate), stats});
+    ctx->save_for_backward({stream, post_w || gate ? b2 : torch::Tensor(), w, or_none(post_w), or_none(post_b), or_none(gate), stats});
     ctx->saved_data["args"] = c10::ivalue::Tuple::create({div, mode, scale, layer, one_plus});
     ctx->saved_data["has"] = c10::ivalue::Tuple::create({b.has_value(), post_w.has_value(), post_b.has_value(), gate.has_value()});
     ctx->set_materialize_grads(false);
@@ -116,8 +122,10 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const Opt dbranch = like(!alike && ctx->needs_input_grad(1), stream), dw = like(ctx->needs_input_grad(2), w);
     const Opt db = like(next_needed(0), w), dpw = like(next_needed(1), s[3]), dpb = like(next_needed(2), s[4]);
     const Opt dg = like(next_needed(3), s[5]);
-    residual_norm_bwd(rows(grads[0]), rows(grads[1]), stream, s[1].defined() ? s[1] : stream, w, opt(s[3]), opt(s[4]), opt(s[5]), div,
-                      mode, scale, args[3].toBool(), args[4].toBool(), s[6], dx, dbranch, dw, db, dpw, dpb, dg);
+    const torch::Tensor s2 = rows_of(stream);
+    residual_norm_bwd(rows(grads[0]), rows(grads[1]), s2, s[1].defined() ? s[1] : s2, w, opt(s[3]), opt(s[4]),
+                      gate_rows(opt(s[5])), div, mode, scale, args[3].toBool(), args[4].toBool(), s[6], rows_of(dx),
+                      dbranch ? Opt(rows_of(*dbranch)) : dbranch, dw, db, dpw, dpb, gate_rows(dg));
     if (ctx->needs_input_grad(0)) out[0] = dx;
     if (ctx->needs_input_grad(1)) out[1] = alike ? dx : *dbranch;
     if (dw) out[2] = *dw;
@@ -241,23 +249,18 @@ std::tuple<torch::Tensor, torch::Tensor> residual_norm(const torch::Tensor& x, c
     for (int64_t i = last + 1; i < lead; ++i) div *= x.size(i);
     mode = last < 0 ? 1 : div == 1 ? 3 : 2;
     div = std::max<int64_t>(div, 1);
-    torch::Tensor t = gate->dim() == 2 ? *gate : gate->reshape({gate->numel() / D, D});
-    g = t.is_contiguous() ? t : t.contiguous();
+    g = gate->is_contiguous() ? *gate : gate->contiguous();
   }
-  const torch::Tensor x2 = rows_of(x), b2 = rows_of(branch);
-  torch::Tensor stream, normed;
   const int vectors = int(wants_grad(w)) + int(wants_grad(b)) + int(wants_grad(post_w)) + int(wants_grad(post_b));
   if (at::GradMode::is_enabled() && (x.requires_grad() || branch.requires_grad() || vectors || wants_grad(gate))) {
     const int sums = vectors + int(wants_grad(gate) && mode != 3);
     SB_VALUE(residual_norm_bwd_fits(D, sums), "residual_norm: ", sums, " column sums of width ", D, " do not fit the backward pass");
-    const auto r = ResidualNorm::apply(x2, b2, wc, bc, pw, pb, g, div, mode, eps, post_eps, scale, layer, one_plus, round_branch);
-    stream = r[0];
-    normed = r[1];
-  } else {
-    stream = torch::empty(x2.sizes(), x.options());
-    normed = torch::empty(x2.sizes(), x.options());
-    residual_norm_fwd(x2, b2, wc, bc, pw, pb, g, div, eps, post_eps, scale, layer, one_plus, round_branch, stream, normed, {});
+    auto r = ResidualNorm::apply(x, branch, wc, bc, pw, pb, g, div, mode, eps, post_eps, scale, layer, one_plus, round_branch);
+    return {r[0], r[1]};
   }
+  const torch::Tensor x2 = rows_of(x), b2 = rows_of(branch);
+  torch::Tensor stream = torch::empty(x2.sizes(), x.options()), normed = torch::empty(x2.sizes(), x.options());
+  residual_norm_fwd(x2, b2, wc, bc, pw, pb, gate_rows(g), div, eps, post_eps, scale, layer, one_plus, round_branch, stream, normed, {});
   if (x.dim() == 2) return {stream, normed};
   return {stream.view(x.sizes()), normed.view(x.sizes())};
 }

@@ -8,12 +8,14 @@
 //
 // Angles are formed in 64 bits: p * freq / 2 pi, of which only the fraction of a turn goes on to
 // the 32-bit sine and cosine, so that a position of 10^6 is as exact as a small one (in 32 bits it
-// would be off by up to 0.06 rad).  They cost rot / 2 products a token for all its heads, kept in
-// shared memory; there is no table and no largest position.
+// would be off by up to 0.06 rad).  There is no table and no largest position.
 //
-// Every value is read and written once, so memory bounds it.  A block turns `tokens` tokens (one,
-// unless heads are few or narrow); a thread handles chunks of VEC pairs: the two vectors of VEC
-// elements that hold them in either layout, 16 bytes each where sizes and alignment allow it.
+// Every value is read and written once, so memory bounds it.  A thread has one place in the heads of
+// a token, a chunk of VEC pairs (the two vectors of VEC elements that hold them in either layout, 16
+// bytes each where sizes and alignment allow it), and turns it in several heads: it forms its
+// angles once, in registers, behind the loads of its first heads.  Angles shared by a block through
+// shared memory are formed once for all heads, but every load waits at a barrier for them: 8192
+// tokens of 40 heads of 128 took 37 us so, 43 with the first loads before the barrier.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/types.h>
@@ -27,7 +29,8 @@
 namespace sb {
 namespace rotary {
 
-constexpr int MAX_THREADS = 512;
+constexpr int THREADS = 128;
+constexpr int HEADS = 4;  // heads whose loads a thread has under way at once
 
 struct Side {  // q or k
   const void* in;
@@ -45,91 +48,107 @@ struct Args {
   const double* freq;  // [rot / 2]
   float factor;
   int inverse;
-  int64_t tokens;
+  int64_t tokens, threads;  // threads: tokens * lanes * chunks of a head
   int S, d, rot;
-  int per_block;  // tokens of a block
-  int copy;       // 1: the channels from rot on are written too (out of place)
+  int chunks;  // of a head: those that turn, then those that pass through (two vectors each)
+  int lanes;   // threads that share a chunk's heads: lane l has heads l, l + lanes, ...
+  int copy;    // 1: the channels from rot on are written too (out of place)
 };
 
 template <class T, int VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(MAX_THREADS) kernel(const __grid_constant__ Args a) {
-  extern __shared__ float2 cs[];  // [per_block][rot / 2]: cos and sin of each pair
-  const int half = a.rot / 2;
-  const int64_t t0 = int64_t(blockIdx.x) * a.per_block;
-  const int nt = int(min(int64_t(a.per_block), a.tokens - t0));
-  for (int e = threadIdx.x; e < nt * half; e += blockDim.x) {
-    const int t = e / half, i = e - t * half;
-    const int64_t tok = t0 + t;
-    const int64_t b = tok / a.S, s = tok - b * a.S;
+__global__ void __launch_bounds__(THREADS, 6) kernel(const __grid_constant__ Args a) {
+  const int64_t at = int64_t(blockIdx.x) * THREADS + threadIdx.x;
+  if (at >= a.threads) return;
+  int64_t tok, b, s;
+  int j, lane;
+  if (a.threads < (int64_t(1) << 31)) {  // 32-bit divisions are a third of the others
+    const uint32_t r = uint32_t(at) / uint32_t(a.chunks);
+    j = int(uint32_t(at) - r * uint32_t(a.chunks));
+    const uint32_t t = r / uint32_t(a.lanes);
+    lane = int(r - t * uint32_t(a.lanes));
+    const uint32_t bb = t / uint32_t(a.S);
+    tok = t, b = bb, s = t - bb * uint32_t(a.S);
+  } else {
+    const int64_t r = at / a.chunks;
+    j = int(at - r * a.chunks);
+    tok = r / a.lanes;
+    lane = int(r - tok * a.lanes);
+    b = tok / a.S, s = tok - b * a.S;
+  }
+  const int half = a.rot / 2, turned = half / VEC;
+  const int heads = a.q.heads + a.k.heads;
+  // the chunk's two vectors within a head; a chunk that passes through may have but one
+  const bool turns = j < turned;
+  const int g = 2 * (j - turned);
+  const int i0 = !turns ? a.rot + VEC * g : INTERLEAVED ? 2 * VEC * j : VEC * j;
+  const int i1 = !turns || INTERLEAVED ? i0 + VEC : half + VEC * j;
+  const bool two = turns || i1 < a.d;
+  const T* qi = static_cast<const T*>(a.q.in) + b * a.q.in_b + s * a.q.in_s;
+  const T* ki = static_cast<const T*>(a.k.in) + b * a.k.in_b + s * a.k.in_s;
+  T* qo = static_cast<T*>(a.q.out) + b * a.q.out_b + s * a.q.out_s;
+  T* ko = static_cast<T*>(a.k.out) + b * a.k.out_b + s * a.k.out_s;
+  vec::Pack<T, VEC> u[HEADS], v[HEADS];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int n = 0; n < HEADS; ++n) {
+      const int h = h0 + n * a.lanes;
+      if (h < heads) {
+        const T* p = h < a.q.heads ? qi + h * a.q.in_h : ki + (h - a.q.heads) * a.k.in_h;
+        u[n].load(p + i0);
+        if (two) v[n].load(p + i1);
+      }
+    }
+  };
+  load(lane);
+  float c[VEC], sn[VEC];
+  if (turns) {
     int64_t p = a.pos0 + s;
     if (a.pos) {
-      const int64_t at = b * a.pos_b + s * a.pos_s;
-      p = a.pos32 ? int64_t(static_cast<const int*>(a.pos)[at]) : static_cast<const int64_t*>(a.pos)[at];
+      const int64_t e = b * a.pos_b + s * a.pos_s;
+      p = a.pos32 ? int64_t(static_cast<const int*>(a.pos)[e]) : static_cast<const int64_t*>(a.pos)[e];
     }
-    const double turns = double(p) * a.freq[i] * 0.15915494309189533577;  // 1 / (2 pi)
-    float sn, c;
-    sincospif(2.f * float(turns - rint(turns)), &sn, &c);
-    cs[e] = make_float2(c * a.factor, a.inverse ? -sn * a.factor : sn * a.factor);
+#pragma unroll
+    for (int m = 0; m < VEC; ++m) {
+      const double turn = double(p) * a.freq[VEC * j + m] * 0.15915494309189533577;  // 1 / (2 pi)
+      sincospif(2.f * float(turn - rint(turn)), &sn[m], &c[m]);
+      c[m] *= a.factor;
+      sn[m] *= a.inverse ? -a.factor : a.factor;
+    }
   }
-  __syncthreads();
-
-  const int turned = half / VEC;                                // chunks of a head that turn
-  const int rest = a.copy ? (a.d - a.rot) / VEC : 0;            // vectors of a head that pass through
-  const int per_head = turned + (rest + 1) / 2;
-  const int heads = a.q.heads + a.k.heads;
-  const int per_token = heads * per_head;
-  for (int e = threadIdx.x; e < nt * per_token; e += blockDim.x) {
-    const int t = e / per_token;
-    int r = e - t * per_token;
-    int h = r / per_head;
-    const int j = r - h * per_head;
-    const int64_t tok = t0 + t;
-    const int64_t b = tok / a.S, s = tok - b * a.S;
-    const bool isq = h < a.q.heads;
-    const Side& w = isq ? a.q : a.k;
-    if (!isq) h -= a.q.heads;
-    const T* in = static_cast<const T*>(w.in) + b * w.in_b + s * w.in_s + h * w.in_h;
-    T* out = static_cast<T*>(w.out) + b * w.out_b + s * w.out_s + h * w.out_h;
-    vec::Pack<T, VEC> u, v;
-    if (j < turned) {
-      const int iu = INTERLEAVED ? 2 * VEC * j : VEC * j;
-      const int iv = INTERLEAVED ? iu + VEC : half + VEC * j;
-      u.load(in + iu);
-      v.load(in + iv);
-      const float2* c = cs + t * half + VEC * j;
-      if (INTERLEAVED) {
-        // the 2 VEC channels of (u, v) are VEC neighbouring pairs
-        vec::Pack<T, VEC> x, y;
+  for (int h0 = lane; h0 < heads; h0 += HEADS * a.lanes) {
+    if (h0 != lane) load(h0);
 #pragma unroll
-        for (int m = 0; m < VEC; ++m) {
-          const float A = 2 * m < VEC ? u.get(2 * m < VEC ? 2 * m : 0) : v.get(2 * m < VEC ? 0 : 2 * m - VEC);
-          const float B = 2 * m + 1 < VEC ? u.get(2 * m + 1 < VEC ? 2 * m + 1 : 0)
-                                          : v.get(2 * m + 1 < VEC ? 0 : 2 * m + 1 - VEC);
-          const float na = A * c[m].x - B * c[m].y, nb = B * c[m].x + A * c[m].y;
-          if (2 * m < VEC) x.set(2 * m < VEC ? 2 * m : 0, na);
-          else y.set(2 * m < VEC ? 0 : 2 * m - VEC, na);
-          if (2 * m + 1 < VEC) x.set(2 * m + 1 < VEC ? 2 * m + 1 : 0, nb);
-          else y.set(2 * m + 1 < VEC ? 0 : 2 * m + 1 - VEC, nb);
-        }
-        x.store(out + iu);
-        y.store(out + iv);
-      } else {
+    for (int n = 0; n < HEADS; ++n) {
+      const int h = h0 + n * a.lanes;
+      if (h >= heads) break;
+      if (turns) {
+        float x[VEC], y[VEC];
+        u[n].unpack(x);
+        v[n].unpack(y);
+        if (INTERLEAVED) {
+          // the 2 VEC channels of (u, v) are VEC neighbouring pairs
+          auto at2 = [&](int m) -> float& { return m < VEC ? x[m < VEC ? m : 0] : y[m < VEC ? 0 : m - VEC]; };
 #pragma unroll
-        for (int m = 0; m < VEC; ++m) {
-          const float A = u.get(m), B = v.get(m);
-          u.set(m, A * c[m].x - B * c[m].y);
-          v.set(m, B * c[m].x + A * c[m].y);
+          for (int m = 0; m < VEC; ++m) {
+            float &A = at2(2 * m), &B = at2(2 * m + 1);
+            const float na = A * c[m] - B * sn[m];
+            B = B * c[m] + A * sn[m];
+            A = na;
+          }
+        } else {
+#pragma unroll
+          for (int m = 0; m < VEC; ++m) {
+            const float na = x[m] * c[m] - y[m] * sn[m];
+            y[m] = y[m] * c[m] + x[m] * sn[m];
+            x[m] = na;
+          }
         }
-        u.store(out + iu);
-        v.store(out + iv);
+        u[n].pack(x);
+        v[n].pack(y);
       }
-    } else {
-      const int g = 2 * (j - turned);
-      const int at = a.rot + VEC * g;
-      u.load(in + at);
-      if (g + 1 < rest) v.load(in + at + VEC);
-      u.store(out + at);
-      if (g + 1 < rest) v.store(out + at + VEC);
+      T* o = h < a.q.heads ? qo + h * a.q.out_h : ko + (h - a.q.heads) * a.k.out_h;
+      u[n].store(o + i0);
+      if (two) v[n].store(o + i1);
     }
   }
 }
@@ -144,16 +163,10 @@ static bool fits(const torch::Tensor& t, int64_t vec) {
 
 template <class T, int VEC>
 static void launch(const Args& a, bool interleaved, cudaStream_t stream) {
-  const int half = a.rot / 2;
-  const int64_t items = int64_t(a.q.heads + a.k.heads) * (half / VEC + ((a.copy ? (a.d - a.rot) / VEC : 0) + 1) / 2);
-  const int threads = int(std::min<int64_t>(MAX_THREADS, std::max<int64_t>(64, (std::max<int64_t>(items * a.per_block, half) + 31) / 32 * 32)));
-  const int64_t blocks = (a.tokens + a.per_block - 1) / a.per_block;
+  const int64_t blocks = (a.threads + THREADS - 1) / THREADS;
   SB_CHECK(blocks < (1ll << 31), "rotary: too many tokens");
-  const size_t smem = size_t(a.per_block) * half * sizeof(float2);
-  if (interleaved)
-    kernel<T, VEC, true><<<dim3(unsigned(blocks)), dim3(threads), smem, stream>>>(a);
-  else
-    kernel<T, VEC, false><<<dim3(unsigned(blocks)), dim3(threads), smem, stream>>>(a);
+  if (interleaved) kernel<T, VEC, true><<<dim3(unsigned(blocks)), THREADS, 0, stream>>>(a);
+  else kernel<T, VEC, false><<<dim3(unsigned(blocks)), THREADS, 0, stream>>>(a);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -232,13 +245,13 @@ void rotary_fwd(const torch::Tensor& q, const c10::optional<torch::Tensor>& k, c
   while (vec > 1 && ((rot / 2) % vec || d % vec || !rotary::fits(q, vec) || !rotary::fits(q_out, vec) ||
                      (k && (!rotary::fits(*k, vec) || !rotary::fits(*k_out, vec)))))
     vec /= 2;
-  // tokens of a block: one while a token fills it, more when its chunks are fewer than 256, as long
-  // as every SM still has several blocks and the angles fit 32 KB
-  const int64_t items = int64_t(heads) * ((rot / 2) / vec + ((d - rot) / vec + 1) / 2);
-  int64_t per = std::max<int64_t>(1, 256 / items);
-  per = std::min<int64_t>(per, std::max<int64_t>(1, a.tokens / (148 * 4)));
-  per = std::min<int64_t>(per, std::max<int64_t>(1, 32768 / (rot / 2 * int64_t(sizeof(float2)))));
-  a.per_block = int(per);
+  a.chunks = int((rot / 2) / vec + (a.copy ? ((d - rot) / vec + 1) / 2 : 0));
+  // a thread turns its chunk in HEADS heads, in fewer where that leaves SMs short of threads
+  const int64_t wave = 148 * 1024;
+  int64_t lanes = (heads + rotary::HEADS - 1) / rotary::HEADS;
+  while (lanes < heads && a.tokens * a.chunks * lanes < wave) lanes = std::min<int64_t>(heads, 2 * lanes);
+  a.lanes = int(lanes);
+  a.threads = a.tokens * a.chunks * lanes;
   const at::cuda::CUDAGuard guard(q.device());
   auto stream = at::cuda::getCurrentCUDAStream();
   if (type == at::kBFloat16) rotary::launch_vec<__nv_bfloat16>(a, vec, interleaved, stream);

@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace sb {
 namespace vec {
 
@@ -31,6 +33,24 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 // the value that T holds for v
 template <class T>
 __device__ __forceinline__ float rounded(float v) { return to_f<T>(from_f<T>(v)); }
+
+// two 16-bit values in one word
+template <class T>
+__device__ __forceinline__ float2 pair_to_f(uint32_t w) {
+  if constexpr (sizeof(T) != 2) return make_float2(0.f, 0.f);
+  else if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pair_from_f(float lo, float hi) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
 
 template <int BYTES>
 struct Raw;
@@ -67,6 +87,31 @@ struct Pack {
     } else {
 #pragma unroll
       for (int i = 0; i < kBytes / 4; ++i) w[i] = 0u;
+    }
+  }
+  // All values at once: 16-bit ones are converted in pairs, one instruction for two on the way back.
+  __device__ __forceinline__ void unpack(float (&f)[VEC]) const {
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(r);
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) {
+        const float2 p = pair_to_f<T>(w[j]);
+        f[2 * j] = p.x;
+        f[2 * j + 1] = p.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = get(j);
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&f)[VEC]) {
+    if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(r);
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) w[j] = pair_from_f<T>(f[2 * j], f[2 * j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) set(j, f[j]);
     }
   }
   __device__ __forceinline__ float get(int j) const { return to_f<T>(reinterpret_cast<const T*>(r)[j]); }
