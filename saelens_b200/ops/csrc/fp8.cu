@@ -19,7 +19,6 @@
 #include <torch/types.h>
 
 #include <algorithm>
-#include <atomic>
 #include <tuple>
 
 #include "block_ops.h"
@@ -278,8 +277,7 @@ struct Prod {
 // features and a part of the reduction; the blocks of a cluster hold the parts of the same features.
 // Column c of the sums belongs to block c % splits: every block writes its part of it there, over
 // distributed shared memory, and after one cluster barrier the owner adds the parts in block order.
-// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)  Two blocks
-// share an SM, half its shared memory each: the grid then fills it with finer parts.
+// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)
 //   warp 0      weight tiles by TMA (and x tiles and scales, unless they are quantised here)
 //   warp 1      tcgen05.mma, 4 a block of 128
 //   warps 2..5  scaled sums in registers: a feature a thread, NT columns
@@ -902,18 +900,10 @@ static CUtensorMap weight_map(const Weight& w, int box_features) {
                       CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// All of an SM's shared memory, asked for: left to itself the runtime divides it for one block, and two
-// that would fit run after one another.
-template <class K>
-static void set_shared(K kern, int smem) {
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-}
-
 template <class K>
 static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st,
                    const CUtensorMap& tW, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a) {
-  set_shared(kern, smem);
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = grid;
@@ -939,39 +929,12 @@ static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool d
 constexpr int FEW = 64;         // rows up to which the few-rows kernel runs
 constexpr int FUSED_ROWS = 2;  // rows up to which it quantises them itself (of 4096 -> 6144: 2 rows 12 us, apart 14.6; 4 rows 17 against 14)
 
-// How many clusters of `size` blocks run at once (asked for once for each shape of kernel and device).
-template <int NT, bool FUSED, class K>
-static int clusters_at_once(K kern, int size, int threads, int smem, int device) {
-  constexpr int DEVICES = 32;
-  static std::atomic<int> known[DEVICES][9];
-  std::atomic<int>* cell = device < DEVICES ? &known[device][size] : nullptr;
-  if (cell && cell->load()) return cell->load();
-  set_shared(kern, smem);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = size;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(size);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-  n = std::max(1, n);
-  if (cell) cell->store(n);
-  return n;
-}
-
-// Parts of the reduction: the most, up to 8, with which all clusters run at once.  A second wave of a
-// few clusters cost as much as the first (48 feature tiles in 6 parts: 12.6 us, in one wave 8).
-template <int NT, bool FUSED, class K>
-static int splits_for(K kern, int64_t feature_tiles, int64_t reduction_blocks, int threads, int smem, int device) {
-  for (int s = int(std::min<int64_t>(8, reduction_blocks)); s > 1; --s)
-    if (feature_tiles * s <= 512 && feature_tiles <= clusters_at_once<NT, FUSED>(kern, s, threads, smem, device)) return s;
-  return 1;
+// Parts of the reduction: up to 8, and 256 blocks in all.  Blocks of half an SM's shared memory follow
+// one another on it without a gap, so more parts than SMs pay until the clusters no longer fit side by
+// side: 48 feature tiles of 32 blocks take 14.8, 11.2, 10.9, 10.6, 10.6, 12.9 us in 1 to 6 parts, 32
+// tiles of 112 blocks 43, 29, 25, 22, 22, 21 and in 8 21; 224 tiles 25 us in one part, 29 in two.
+static int splits_for(int64_t feature_tiles, int64_t reduction_blocks) {
+  return int(std::max<int64_t>(1, std::min<int64_t>({256 / feature_tiles, 8, reduction_blocks})));
 }
 
 template <int NT, bool FUSED, class TX, class TO>
@@ -981,7 +944,7 @@ static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& 
   const CUtensorMap tW = weight_map(w, BLK);
   const int threads = FUSED ? 320 : 192, smem = Few<NT>::SMEM;
   auto go = [&](auto kern) {
-    a.splits = splits_for<NT, FUSED>(kern, tiles, (w.R + BLK - 1) / BLK, threads, smem, c10::cuda::current_device());
+    a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK);
     launch(kern, dim3(unsigned(tiles * a.splits)), threads, smem, a.splits, a.dependent, st, tW, tX, tS, a);
   };
   if constexpr (FUSED) {
@@ -1059,11 +1022,14 @@ static void linear_t(const torch::Tensor& x, const Weight& w, Prod a, cudaStream
     return;
   }
   const int64_t ldq = up(w.R, 16), lds = up(a.M, 4), RB = (w.R + BLK - 1) / BLK;
-  torch::Tensor q = torch::empty({a.M * ldq}, x.options().dtype(at::kByte));
-  torch::Tensor s = torch::empty({RB * lds}, x.options().dtype(at::kFloat));
-  quantize_rows(x, q.data_ptr<uint8_t>(), ldq, s.data_ptr<float>(), lds, st);
+  // one allocation: the values, then the scales
+  const int64_t values = up(a.M * ldq, 256);
+  torch::Tensor held = torch::empty({values + RB * lds * 4}, x.options().dtype(at::kByte));
+  uint8_t* q = held.data_ptr<uint8_t>();
+  float* s = reinterpret_cast<float*>(q + values);
+  quantize_rows(x, q, ldq, s, lds, st);
   a.dependent = 1;  // the quantisation itself began after everything before it had ended
-  product<T>(q.data_ptr<uint8_t>(), ldq, s.data_ptr<float>(), lds, w, a, st);
+  product<T>(q, ldq, s, lds, w, a, st);
 }
 
 }  // namespace fp8
