@@ -19,7 +19,9 @@
 #include <torch/types.h>
 
 #include <algorithm>
+#include <atomic>
 #include <tuple>
+#include <type_traits>
 
 #include "block_ops.h"
 #include "check.h"
@@ -97,22 +99,21 @@ __device__ __forceinline__ float half_warp_most(const float (&v)[8]) {
   return __uint_as_float(m);
 }
 
-// Rows: a half-warp quantises a row's 128 values, 8 a lane; 16 rows a block, `per` blocks of 128 a
-// half-warp (at most QPER, all loads issued before the first maximum).  Memory-bound: 2 bytes read
-// and 1 written a value.
-constexpr int QPER = 4;
-template <class T, bool ALIGNED>
+// Rows: a half-warp quantises a row's 128 values, 8 a lane; 16 rows a block, PER blocks of 128 a
+// half-warp (all loads issued before the first maximum).  Memory-bound: 2 bytes read and 1 written
+// a value.
+template <class T, bool ALIGNED, int PER>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int64_t K,
                                                             uint8_t* __restrict__ q, int64_t ldq,
-                                                            float* __restrict__ scale, int64_t lds, int per) {
+                                                            float* __restrict__ scale, int64_t lds) {
   asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 15;
   const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
-  const int64_t kb0 = int64_t(blockIdx.y) * per, KB = (K + BLK - 1) / BLK;
-  float v[QPER][8];
+  const int64_t kb0 = int64_t(blockIdx.y) * PER, KB = (K + BLK - 1) / BLK;
+  float v[PER][8];
 #pragma unroll
-  for (int i = 0; i < QPER; ++i) {
-    if (i < per && kb0 + i < KB && row < M) {
+  for (int i = 0; i < PER; ++i) {
+    if (kb0 + i < KB && row < M) {
       load8<T, ALIGNED>(x + row * ldx, (kb0 + i) * BLK + lane * 8, K, v[i]);
     } else {
 #pragma unroll
@@ -120,8 +121,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
     }
   }
 #pragma unroll
-  for (int i = 0; i < QPER; ++i) {
-    if (i >= per) break;  // uniform
+  for (int i = 0; i < PER; ++i) {
     const float most = half_warp_most(v[i]);
     const int64_t kb = kb0 + i, c = kb * BLK + lane * 8;
     if (row < M && kb < KB) {
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
 
 // ---- many rows ------------------------------------------------------------------------------
 // Persistent; PAIR: two SMs (a cluster of 2) share a 256 x 256 tile by one cta_group::2 product, each
-// staging half of either operand, else one SM has a 128 x 128 tile.  A stage's bytes pass shared
+// staging half of either operand, else one SM has a 128 x 128 or 128 x 256 tile.  A stage's bytes pass shared
 // memory twice, written by TMA and read by the tensor core: 64 KB for 512 cycles of products in a
 // pair, 96 KB on one SM with a 128 x 256 tile, which that bounds.  Every block of 128 of the
 // reduction goes to one of two TMEM accumulators.
@@ -824,18 +824,37 @@ static void check_rows(const torch::Tensor& x, const char* what) {
   SB_CHECK(x.size(1) >= 1 && x.size(0) < (1ll << 31) - 256 && x.size(1) < (1ll << 31) - 256, what, ": size");
 }
 
+// Kernel attributes are set once for each kernel (K is its address) and device.
+template <auto K>
+static void set_once(cudaFuncAttribute what, int value) {
+  static std::atomic<uint64_t> done{0};
+  const int device = c10::cuda::current_device();
+  const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+  if (done.load() & bit) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(K, what, value));
+  done.fetch_or(bit);
+}
+
 template <class T>
 static void quantize_rows_t(const torch::Tensor& x, uint8_t* q, int64_t ldq, float* s, int64_t lds, cudaStream_t st) {
   const int64_t M = x.size(0), K = x.size(1), KB = (K + BLK - 1) / BLK;
   const int64_t rb = (M + 15) / 16;
   // several blocks of 128 a half-warp once there are blocks for every SM without
-  const int per = rb * KB >= 148 * 8 * QPER ? QPER : 1;
+  const int per = rb * KB >= 148 * 8 * 4 ? 4 : 1;
   const int64_t ny = (KB + per - 1) / per;
   SB_CHECK(ny <= 65535, "quantize_fp8: rows of more than 8 million values");
   const dim3 grid{unsigned(rb), unsigned(ny)};
   const T* p = static_cast<const T*>(x.data_ptr());
-  if (rows_aligned(x)) quantize_rows_kernel<T, true><<<grid, 256, 0, st>>>(p, x.stride(0), M, K, q, ldq, s, lds, per);
-  else quantize_rows_kernel<T, false><<<grid, 256, 0, st>>>(p, x.stride(0), M, K, q, ldq, s, lds, per);
+  auto go = [&](auto aligned, auto n) {
+    constexpr auto kern = quantize_rows_kernel<T, decltype(aligned)::value, decltype(n)::value>;
+    // The SM's memory is divided as the product's blocks want it, or none of them starts beside this kernel.
+    set_once<kern>(cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    kern<<<grid, 256, 0, st>>>(p, x.stride(0), M, K, q, ldq, s, lds);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  if (rows_aligned(x)) per == 1 ? go(std::true_type{}, One{}) : go(std::true_type{}, Four{});
+  else per == 1 ? go(std::false_type{}, One{}) : go(std::false_type{}, Four{});
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -900,10 +919,10 @@ static CUtensorMap weight_map(const Weight& w, int box_features) {
                       CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <class K>
-static void launch(K kern, dim3 grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st,
+template <auto kern>
+static void launch(dim3 grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st,
                    const CUtensorMap& tW, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a) {
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  set_once<kern>(cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = grid;
@@ -943,19 +962,18 @@ static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& 
   SB_CHECK(tiles < (1ll << 27), "fp8 product: size of the weight");
   const CUtensorMap tW = weight_map(w, BLK);
   const int threads = FUSED ? 320 : 192, smem = Few<NT>::SMEM;
-  auto go = [&](auto kern) {
-    a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK);
-    launch(kern, dim3(unsigned(tiles * a.splits)), threads, smem, a.splits, a.dependent, st, tW, tX, tS, a);
+  a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK);
+  auto go = [&](auto aligned, auto mn) {
+    launch<few_rows_kernel<NT, FUSED, decltype(aligned)::value, decltype(mn)::value, TX, TO>>(
+        dim3(unsigned(tiles * a.splits)), threads, smem, a.splits, a.dependent, st, tW, tX, tS, a);
   };
   if constexpr (FUSED) {
     if (!x_aligned) {
-      if (w.mn) go(few_rows_kernel<NT, true, false, true, TX, TO>);
-      else go(few_rows_kernel<NT, true, false, false, TX, TO>);
+      w.mn ? go(std::false_type{}, std::true_type{}) : go(std::false_type{}, std::false_type{});
       return;
     }
   }
-  if (w.mn) go(few_rows_kernel<NT, FUSED, true, true, TX, TO>);
-  else go(few_rows_kernel<NT, FUSED, true, false, TX, TO>);
+  w.mn ? go(std::true_type{}, std::true_type{}) : go(std::true_type{}, std::false_type{});
 }
 
 template <bool PAIR, int BN, class TO>
@@ -967,8 +985,8 @@ static void many_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap&
   const dim3 grid{unsigned(PAIR ? 2 * std::min<int64_t>(tiles, sms / 2) : std::min<int64_t>(tiles, sms))};
   const CUtensorMap tW = weight_map(w, C::W_ROWS);
   const int cluster = PAIR ? 2 : 1;
-  if (w.mn) launch(many_rows_kernel<PAIR, BN, true, TO>, grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
-  else launch(many_rows_kernel<PAIR, BN, false, TO>, grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
+  if (w.mn) launch<many_rows_kernel<PAIR, BN, true, TO>>(grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
+  else launch<many_rows_kernel<PAIR, BN, false, TO>>(grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
 }
 
 // Quantised rows (uint8 [M, R] with row stride ldq) and their scales ([blocks][lds]) times the weight.
@@ -983,9 +1001,13 @@ static void product(const uint8_t* q, int64_t ldq, const float* scales, int64_t 
   else if (a.M <= FEW) few_rows<64, false, float, TO>(w, tX, tS, a, true, st);
   else {
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-    const int64_t pairs = ((a.M + 255) / 256) * ((w.F + 255) / 256);
-    if (pairs >= sms / 4) many_rows<true, 256, TO>(w, tX, tS, a, st);
-    else many_rows<false, 128, TO>(w, tX, tS, a, st);
+    // While one wave of SMs holds all tiles, the time is that of one tile: 0.37 us a block of 128 for 128
+    // features, 0.49 for 256, 0.54 for a pair's (333 x 5120 -> 7168: 44, 29 and 31 us).  Beyond, a pair's
+    // tile costs least for its size (2048 x 4096 -> 14336: 176, 146 and 137 us).
+    const int64_t m = (a.M + 127) / 128;
+    if (m * ((w.F + 127) / 128) <= sms) many_rows<false, 128, TO>(w, tX, tS, a, st);
+    else if (m * ((w.F + 255) / 256) <= sms) many_rows<false, 256, TO>(w, tX, tS, a, st);
+    else many_rows<true, 256, TO>(w, tX, tS, a, st);
   }
 }
 
