@@ -305,6 +305,7 @@ def _fuses_residual(x: torch.Tensor, out: torch.Tensor, post: Norm | None, hook_
     """Whether one kernel may do the residual update and the norms around it: inference on CUDA in a
     type that the single norms run on, nothing reading in between."""
     return (_native_ok(x) and x.dtype in (torch.bfloat16, torch.float32) and out.dtype == x.dtype == then.w.dtype
+            and x.is_contiguous() and out.is_contiguous()
             and 8 <= cfg.d_model <= 16384 and cfg.d_model % 8 == 0 and _plain(hook_out) and _plain(hook_stream)
             and _unwatched(then)
             and (post is None or (post.w.dtype == x.dtype and _unwatched(post) and _plain(post.hook_normalized))))

@@ -142,6 +142,30 @@ torch::Tensor last_contiguous(const torch::Tensor& t) {
   return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
 
+// Whether q and k of one storage may hold a value in common.  Views of one tensor have the same strides
+// between sequences and tokens: they are apart if what they span of a sequence or of a token is, or if
+// their heads interleave with one stride and never meet.  Others are apart if all they span is.
+bool may_share(const torch::Tensor& q, const torch::Tensor& k) {
+  if (q.numel() == 0 || k.numel() == 0 || q.storage().data_ptr().get() != k.storage().data_ptr().get()) return false;
+  const int64_t d = q.size(3), oq = q.storage_offset(), ok = k.storage_offset();
+  auto span = [](const torch::Tensor& t, int from) {
+    int64_t n = 1;
+    for (int i = from; i < 4; ++i) n += (t.size(i) - 1) * t.stride(i);
+    return n;
+  };
+  if (oq + span(q, 0) <= ok || ok + span(k, 0) <= oq) return false;
+  for (int i = 0; i < 2; ++i) {
+    // what one entry of dimension i spans; it must not reach into the next one's for this to say anything
+    const int64_t eq = oq + span(q, i + 1), ek = ok + span(k, i + 1);
+    if (q.size(i) > 1 && (q.stride(i) != k.stride(i) || std::max(eq, ek) - std::min(oq, ok) > q.stride(i))) return true;
+    if (eq <= ok || ek <= oq) return false;
+  }
+  const int64_t step = q.size(2) > 1 ? q.stride(2) : k.stride(2);
+  if ((q.size(2) > 1 && k.size(2) > 1 && q.stride(2) != k.stride(2)) || step < 2 * d) return true;
+  const int64_t apart = ((ok - oq) % step + step) % step;
+  return apart < d || apart > step - d;
+}
+
 std::tuple<torch::Tensor, torch::Tensor> turn(const torch::Tensor& q0, const torch::Tensor& k0, const torch::Tensor& freq,
                                               const Opt& pos, int64_t offset, bool interleaved, bool inverse, double factor) {
   const torch::Tensor q = last_contiguous(q0);
@@ -299,7 +323,10 @@ std::tuple<torch::Tensor, Opt> rotary(const torch::Tensor& q, const Opt& k, cons
       SB_VALUE(ok, "rotary: in place needs contiguous channels and no value twice");
     };
     check(q);
-    if (k) check(*k);
+    if (k) {
+      check(*k);
+      SB_VALUE(!may_share(q, *k), "rotary: in place, q and k must not share values");
+    }
     rotary_fwd(q, k, f, pos, offset, interleaved, false, factor, q, k);
     return {q, k};
   }

@@ -170,6 +170,28 @@ def test_beyond_32_bit_offsets():
         check(out[:, a:b], q[:, a:b], torch.arange(a, b, device="cuda")[None], f, False)
 
 
+def test_in_place_on_views_of_one_tensor():
+    """q and k may interleave head by head, but not hold a value in common."""
+    from saelens_b200 import ops
+
+    f = freqs(64)
+    pairs = torch.randn(2, 5, 4, 2, 64, device="cuda")
+    q, k = pairs[..., 0, :], pairs[..., 1, :]
+    want = ops.rotary(q, k, f)
+    ops.rotary(q, k, f, inplace=True)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    halves = torch.randn(2, 10, 4, 64, device="cuda")
+    q, k = halves[:, :5], halves[:, 5:]
+    want = ops.rotary(q, k, f)
+    ops.rotary(q, k, f, inplace=True)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+    x = torch.randn(2, 5, 4, 64, device="cuda")
+    for q, k in ((x, x), (x[:, :, :3], x[:, :, 1:]), (x, x[:, :, 3:]), (x[:, :4], x[:, 1:]), (x[..., :34], x[..., 30:])):
+        with pytest.raises(ValueError, match="share"):
+            ops.rotary(q, k, freqs(32), inplace=True)
+    ops.rotary(x[:, :, :3], x[:, :, 3:], f, inplace=True)
+
+
 def test_refusals_on_the_device():
     from saelens_b200 import ops
 
