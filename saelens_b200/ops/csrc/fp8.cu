@@ -42,26 +42,18 @@ constexpr uint32_t LEAST_BITS = 0x04e00000u;  // 448 * 2^-126
 // Bit patterns of absolute values order like the values, with NaN above infinity: a NaN stays.
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-__device__ __forceinline__ float quotient(float v, float most) { return v * 0.4375f / most * 1024.f; }
-
-// e4m3 of 448 v / most.  A product with 448 / most is off by less than 8 units in the last place of
-// fp32, so it rounds to the same e4m3 value unless that many from a border (the 20 bits behind the 3
-// that e4m3 keeps are near 0x80000) or below 2^-6, where e4m3's steps are no longer relative; only
-// then the quotient is formed.  Dividing every value made the quantisation issue-bound: 41 us for
-// 8192 x 4096 values, whose bytes take 15.
-__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float most) {
-  const float by = MAXV / most;
+// e4m3 of 448 v / most, the quotient rounded once.  t is the product with a rounded reciprocal; its
+// exact residual, which one fused multiply-add gives, times that reciprocal makes it the correctly
+// rounded quotient (Markstein 1990).  A division for every value made the quantisation issue-bound (41
+// us for 8192 x 4096 values, whose bytes take 15), and one only for values near a border of e4m3 little
+// less: of 16-bit values many lie on one.  Scaled by 1024 so that the reciprocal stays a normal
+// number; an infinite maximum gives NaN.
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], float most, float by) {  // by = 1024 / most
   float t[8];
-  bool near = false;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    t[j] = v[j] * by;
-    const uint32_t b = abs_bits(t[j]);
-    near = near || ((b - (0x80000u - 8u)) & 0xfffffu) <= 16u || (b < 0x3c800000u && b != 0u);
-  }
-  if (near) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = quotient(v[j], most);
+    const float num = v[j] * 0.4375f, q = num * by;
+    t[j] = __fmaf_rn(__fmaf_rn(q * -0.0009765625f, most, num), by, q);
   }
   uint32_t w[2];
 #pragma unroll
@@ -76,17 +68,46 @@ __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float most) {
 // 8 values from column c of a row; columns from K on are 0.  ALIGNED: rows start on 16 bytes and K is
 // a multiple of 8.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t K, float (&v)[8]) {
+__device__ __forceinline__ vec::Pack<T, 8> load_pack(const T* row, int64_t c, int64_t K) {
+  vec::Pack<T, 8> p;
+  p.zero();
   if (ALIGNED) {
-    vec::Pack<T, 8> p;
     if (c < K) p.load(row + c);
-    else p.zero();
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = p.get(j);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < K ? vec::to_f<T>(row[c + j]) : 0.f;
+    for (int j = 0; j < 8; ++j)
+      if (c + j < K) reinterpret_cast<T*>(p.r)[j] = row[c + j];
   }
+  return p;
+}
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void load8(const T* row, int64_t c, int64_t K, float (&v)[8]) {
+  load_pack<T, ALIGNED>(row, c, K).unpack(v);
+}
+
+// A key of the largest absolute value of 8: its bits in T, in which two 16-bit values compare at once.
+template <class T>
+__device__ __forceinline__ uint32_t most_key(const vec::Pack<T, 8>& p) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(p.r);
+    uint32_t m = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int j = 1; j < 4; ++j) m = __vmaxu2(m, w[j] & 0x7fff7fffu);
+    return max(m & 0xffffu, m >> 16);
+  } else {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(p.get(j)));
+    return m;
+  }
+}
+// The value of a key, LEAST at least.
+template <class T>
+__device__ __forceinline__ float key_value(uint32_t key) {
+  uint32_t bits = key;
+  if constexpr (std::is_same_v<T, __half>) bits = __float_as_uint(__half2float(__ushort_as_half(uint16_t(key))));
+  else if constexpr (sizeof(T) == 2) bits = key << 16;
+  return __uint_as_float(max(bits, LEAST_BITS));
 }
 
 // The largest absolute value (as bits, at least LEAST_BITS) of the 16 lanes of a half-warp.
@@ -110,24 +131,28 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
   const int lane = threadIdx.x & 15;
   const int64_t row = int64_t(blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int64_t kb0 = int64_t(blockIdx.y) * PER, KB = (K + BLK - 1) / BLK;
-  float v[PER][8];
+  const T* from = x + (row < M ? row : 0) * ldx;
+  vec::Pack<T, 8> p[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) p[i] = load_pack<T, ALIGNED>(from, (kb0 + i) * BLK + lane * 8, row < M ? K : 0);
+  uint32_t key[PER], mine = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    if (kb0 + i < KB && row < M) {
-      load8<T, ALIGNED>(x + row * ldx, (kb0 + i) * BLK + lane * 8, K, v[i]);
-    } else {
+    key[i] = most_key<T>(p[i]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    }
+    for (int o = 8; o > 0; o >>= 1) key[i] = max(key[i], __shfl_xor_sync(0xffffffffu, key[i], o));
+    if ((lane & (PER - 1)) == i) mine = key[i];
   }
+  // lane i divides for block i (lanes from PER on again), and the others take the reciprocal from it
+  const float most = key_value<T>(mine), by = 1024.f / most;
+  if (lane < PER && row < M && kb0 + lane < KB) scale[(kb0 + lane) * lds + row] = most / MAXV;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const float most = half_warp_most(v[i]);
-    const int64_t kb = kb0 + i, c = kb * BLK + lane * 8;
-    if (row < M && kb < KB) {
-      if (c < ldq) *reinterpret_cast<uint2*>(q + row * ldq + c) = quantize8(v[i], most);
-      if (lane == 0) scale[kb * lds + row] = most / MAXV;
-    }
+    const int64_t c = (kb0 + i) * BLK + lane * 8;
+    const float r = __shfl_sync(0xffffffffu, by, (threadIdx.x & 16) + i);
+    float v[8];
+    p[i].unpack(v);
+    if (row < M && c < ldq) *reinterpret_cast<uint2*>(q + row * ldq + c) = quantize8(v, key_value<T>(key[i]), r);
   }
 }
 
@@ -159,11 +184,11 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const T* __restric
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, red[i]);
-  const float most = __uint_as_float(m);
+  const float most = __uint_as_float(m), by = 1024.f / most;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t row = nb * BLK + i * 16 + (threadIdx.x >> 4);
-    if (row < N && c < ldq) *reinterpret_cast<uint2*>(q + row * ldq + c) = quantize8(v[i], most);
+    if (row < N && c < ldq) *reinterpret_cast<uint2*>(q + row * ldq + c) = quantize8(v[i], most, by);
   }
   if (threadIdx.x == 0) scale[nb * gridDim.x + kb] = most / MAXV;
 }
@@ -458,7 +483,7 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
       const bool have = i < items;
       const int j = have ? i / a.M : 0, m = have ? i - j * a.M : 0;
       const float most = half_warp_most(v);
-      const uint2 w = quantize8(v, most);
+      const uint2 w = quantize8(v, most, 1024.f / most);
       load_item(i + 8);  // the next one's values arrive meanwhile
       const int s = j % C::STAGES, g = j % C::RING;
       bool ok = true;
@@ -840,7 +865,7 @@ static void quantize_rows_t(const torch::Tensor& x, uint8_t* q, int64_t ldq, flo
   const int64_t M = x.size(0), K = x.size(1), KB = (K + BLK - 1) / BLK;
   const int64_t rb = (M + 15) / 16;
   // several blocks of 128 a half-warp once there are blocks for every SM without
-  const int per = rb * KB >= 148 * 8 * 4 ? 4 : 1;
+  const int per = rb * KB >= 148 * 8 * 2 ? 4 : 1;
   const int64_t ny = (KB + per - 1) / per;
   SB_CHECK(ny <= 65535, "quantize_fp8: rows of more than 8 million values");
   const dim3 grid{unsigned(rb), unsigned(ny)};
