@@ -12,7 +12,9 @@
 //     dx = dr + dpre,  du = scale gate dx,  dgate = sum of scale dx u,  dbranch = dpost(du).
 //
 // Memory bounds both directions: forward reads x and branch and writes r and y, backward reads
-// dr, dy, r and the branch where it is needed, and writes dx and dbranch.  A row is held in the
+// dr, dy, r and the branch where it is needed, and writes dx and dbranch.  8192 bf16 rows of 4096 go
+// forward in 42 us (6.3 TB/s), with a post-norm in 48; backward, which also waits for its rows and
+// adds column sums, in 79 (3.4 TB/s) and 137.  A row is held in the
 // registers of one block between the sums, so every value moves once.  Sums are 32-bit and
 // deterministic: thread t holds the vectors t, t + threads, ..., lanes are joined by a butterfly
 // and warps in order, and a layer norm's weight and bias enter as one fused multiply-add, as in the
@@ -253,7 +255,8 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int tid, int
 // A block is `groups` groups of threads, each with rows of its own.  Where a thread has one vector
 // (rows of up to 2048 values) its column sums stay in registers and a block has several groups, so
 // that rows wait for their sums side by side and there are few blocks' sums to join; wider rows keep
-// theirs in shared memory, one group a block.  4104 fp32 rows of 768 with five sums: 39 -> 17 us.
+// theirs in shared memory, one group a block.  4104 fp32 rows of 768 with five sums: 39 -> 30 us, and
+// the sums' join 10 -> 6.
 constexpr int GROUP_THREADS = 512;
 template <class T, int VEC, int NV, bool LAYER, bool POST>
 __global__ void __launch_bounds__(NV == 1 ? GROUP_THREADS : THREADS) bwd_kernel(const __grid_constant__ Bwd a) {

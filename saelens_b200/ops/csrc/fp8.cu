@@ -250,9 +250,8 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
 __device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
-// mbar_wait_bounded with its clock off the path: a wait is on the way of every block of 128 here, and
-// reading the clock after the first failed try made a block's hand-over several times as long.  The
-// limit is the same.
+// mbar_wait_bounded that reads the clock only after 64 tries: a wait is on the way of every block of
+// 128 here, and most end within the first.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort, int* status, int code) {
   for (int i = 0; i < 64; ++i)
     if (mbar_try_wait(bar, parity)) return true;
@@ -302,7 +301,9 @@ struct Prod {
 // features and a part of the reduction; the blocks of a cluster hold the parts of the same features.
 // Column c of the sums belongs to block c % splits: every block writes its part of it there, over
 // distributed shared memory, and after one cluster barrier the owner adds the parts in block order.
-// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)
+// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)  One row 4096 ->
+// 6144 8.0 us, 24 rows 14336 -> 4096 18.0 with their quantisation (25 and 59 MB of weight: 3.9 and 9.0
+// us at the copy rate); what remains is launch, the first bytes' latency and the cluster's barrier.
 //   warp 0      weight tiles by TMA (and x tiles and scales, unless they are quantised here)
 //   warp 1      tcgen05.mma, 4 a block of 128
 //   warps 2..5  scaled sums in registers: a feature a thread, NT columns
@@ -543,10 +544,13 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
 
 // ---- many rows ------------------------------------------------------------------------------
 // Persistent; PAIR: two SMs (a cluster of 2) share a 256 x 256 tile by one cta_group::2 product, each
-// staging half of either operand, else one SM has a 128 x 128 or 128 x 256 tile.  A stage's bytes pass shared
-// memory twice, written by TMA and read by the tensor core: 64 KB for 512 cycles of products in a
+// staging half of either operand, else one SM has a 128 x 128 or 128 x 256 tile.  A stage's bytes pass
+// shared memory twice, written by TMA and read by the tensor core: 64 KB for 512 cycles of products in a
 // pair, 96 KB on one SM with a 128 x 256 tile, which that bounds.  Every block of 128 of the
-// reduction goes to one of two TMEM accumulators.
+// reduction goes to one of two TMEM accumulators, and the hand-over between products and sums is what
+// a block costs: 840 cycles a pair's, of which the products are 541 (without any scaling 690).  Under
+// sustained load the 1 kW limit binds: 77% of the same kernel's rate without scales.  8192 x 4096 ->
+// 28672 in 0.91 ms of products (2.1 PFLOP/s), 2048 x 4096 -> 14336 in 0.135 (1.8).
 //   warps 0..7   scaled sums in registers: a row a thread, half of the tile's features (warps 0-3 the first)
 //   warp 8       TMA;  warp 9  tcgen05.mma (in the pair's first block);  warps 10, 11 only give up registers
 template <bool PAIR, int BN_>
