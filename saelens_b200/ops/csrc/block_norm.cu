@@ -65,7 +65,11 @@ struct Fwd {
 // What hides the latencies of a row (loads, one to four sums, vectors from the L2 cache) is other rows
 // on the SM, so registers are held to what FWD_BLOCKS blocks leave.
 template <class T, int VEC, int NV>
-constexpr int FWD_BLOCKS = VEC * NV * int(sizeof(T)) <= 16 ? 7 : VEC * NV * int(sizeof(T)) <= 32 ? 6 : VEC * NV * int(sizeof(T)) <= 64 ? 3 : 1;
+constexpr int FWD_BLOCKS = VEC == 1              ? (NV <= 4 ? 6 : NV <= 16 ? 3 : 1)
+                           : NV * int(sizeof(T)) <= 2 ? 7
+                           : NV * int(sizeof(T)) <= 4 ? 6
+                           : NV * int(sizeof(T)) <= 8 ? 3
+                                                      : 1;
 template <class T, int VEC, int NV, bool LAYER, bool POST>
 __global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(const __grid_constant__ Fwd a) {
   __shared__ float red[4][WARPS];

@@ -91,7 +91,8 @@ def test_quantize_strided_and_special_values():
 
 SIZES = [(1, 128, 128), (1, 4096, 640), (1, 28672, 20000), (2, 14336, 8192), (2, 1, 1), (4, 9000, 6150), (5, 130, 129), (16, 1024, 257), (17, 1024, 384), (24, 3584, 520),
          (32, 333, 100), (33, 2048, 1000), (64, 640, 2048), (65, 640, 2048), (127, 100, 300), (129, 1152, 130),
-         (333, 5120, 1111), (1000, 2056, 2304), (2048, 512, 6200)]
+         (333, 5120, 1111), (1000, 2056, 2304), (2048, 512, 6200),
+         (333, 640, 7168), (300, 200, 30000)]
 
 
 @pytest.mark.parametrize("m,k,n", SIZES)
@@ -125,7 +126,8 @@ def test_gemm_of_quantized_rows(m, k, n):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 128, 128), (1, 4096, 640), (3, 130, 129), (16, 256, 1024), (20, 1000, 384),
-                                   (64, 640, 2048), (127, 100, 300), (333, 1111, 5120), (1030, 2304, 2056)])
+                                   (64, 640, 2048), (127, 100, 300), (333, 1111, 5120), (1030, 2304, 2056),
+                                   (2000, 4100, 384)])
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_gradient_of_rows(m, k, n, dtype):
     from saelens_b200 import ops
