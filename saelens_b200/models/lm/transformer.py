@@ -63,15 +63,15 @@ class LMConfig:
     attn_softcap: float | None = None
     final_softcap: float | None = None
     query_pre_attn_scalar: float | None = None
+    model_name: str = "custom"
+    dtype: str = "bfloat16"
+    init_std: float = 0.02
     rotary_dim: int | None = None          # channels of a head that turn (None: all)
     rotary_interleaved: bool = False       # pairs of neighbours instead of the two halves
     rope_scaling: dict[str, Any] | None = None  # stretched context, see ops.rotary_frequencies
     residual_scale: float = 1.0            # what each sub-block adds is multiplied by this
     branch_gate: bool = False              # and by a learned gate per channel
     weight_quantization: str | None = None  # "fp8": the blocks' projections in e4m3 (models/lm/fp8.py)
-    model_name: str = "custom"
-    dtype: str = "bfloat16"
-    init_std: float = 0.02
 
     def __post_init__(self) -> None:
         if self.d_head is None:
