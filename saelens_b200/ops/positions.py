@@ -24,7 +24,8 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict[str, Any] 
     use); "llama3" divides those that turn fewer than `low_freq_factor` times in the original context
     by `factor`, keeps those above `high_freq_factor` and blends between; "yarn" (Peng et al. 2023)
     blends over pairs between `beta_slow` and `beta_fast` turns and puts `attention_factor` (0.1
-    ln(factor) + 1 unless given) on cos and sin; "default" or None keeps them."""
+    ln(factor) + 1 unless given, or the ratio of 0.1 m ln(factor) + 1 for m = `mscale` and
+    `mscale_all_dim`) on cos and sin; "default" or None keeps them."""
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary_frequencies: dim must be even and positive, got {dim}")
     if not base > 0:
@@ -63,8 +64,15 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict[str, Any] 
     lo = max(math.floor(pair_of(float(s.get("beta_fast") or 32.0))), 0)
     hi = min(math.ceil(pair_of(float(s.get("beta_slow") or 1.0))), dim - 1)
     ramp = ((i / 2 - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
+
+    def stretch(m: float) -> float:
+        return 0.1 * m * math.log(factor) + 1.0
+
     attention = s.get("attention_factor")
-    attention = float(attention) if attention is not None else (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+    if attention is None:
+        both = s.get("mscale") and s.get("mscale_all_dim")
+        attention = stretch(float(s["mscale"])) / stretch(float(s["mscale_all_dim"])) if both else stretch(1.0)
+    attention = float(attention)
     return (freq * (1 - ramp) + freq / factor * ramp).to(device), attention
 
 

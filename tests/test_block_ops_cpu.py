@@ -114,6 +114,9 @@ def test_frequencies():
     assert a == pytest.approx(0.1 * math.log(16) + 1, rel=1e-15)
     assert torch.allclose(g[turns > 40], f[turns > 40], rtol=1e-14) and torch.allclose(g[turns < 0.8], f[turns < 0.8] / 16, rtol=1e-14)
     assert ops.rotary_frequencies(128, 10000.0, {**y, "attention_factor": 1.0})[1] == 1.0
+    ratio = (0.0707 * math.log(16) + 1) / (0.1 * math.log(16) + 1)
+    assert ops.rotary_frequencies(128, 10000.0, {**y, "mscale": 0.707, "mscale_all_dim": 1.0})[1] == pytest.approx(ratio, rel=1e-14)
+    assert ops.rotary_frequencies(128, 10000.0, {**y, "factor": 1.0})[1] == 1.0
 
     # with the length: unchanged up to the original context, a larger base beyond
     d = {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 2048}
