@@ -35,10 +35,15 @@
 namespace sb {
 namespace bnorm {
 
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
+constexpr int THREADS = 256;          // of a row in vectors of 8
+constexpr int THREADS_NARROW = 512;   // of a wide row in single values
+template <int VEC>
+constexpr int MAX_THREADS = VEC == 1 ? THREADS_NARROW : THREADS;
+template <int VEC>
+constexpr int WARPS = MAX_THREADS<VEC> / 32;
 
-// Sum over the block; `red` is one of the caller's buffers of WARPS floats, each used once a row.
+// Sum over the block; `red` is one of the caller's buffers of MOST floats, each used once a row.
+template <int MOST>
 __device__ __forceinline__ float block_sum(float v, float* red, int warps) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -46,7 +51,7 @@ __device__ __forceinline__ float block_sum(float v, float* red, int warps) {
   __syncthreads();
   float t = 0.f;
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i)
+  for (int i = 0; i < MOST; ++i)
     if (i < warps) t += red[i];
   return t;
 }
@@ -65,14 +70,14 @@ struct Fwd {
 // What hides the latencies of a row (loads, one to four sums, vectors from the L2 cache) is other rows
 // on the SM, so registers are held to what FWD_BLOCKS blocks leave.
 template <class T, int VEC, int NV>
-constexpr int FWD_BLOCKS = VEC == 1              ? (NV <= 4 ? 6 : NV <= 16 ? 3 : 1)
+constexpr int FWD_BLOCKS = VEC == 1                     ? (NV <= 4 ? 3 : NV <= 8 ? 2 : 1)
                            : NV * int(sizeof(T)) <= 2 ? 7
                            : NV * int(sizeof(T)) <= 4 ? 6
                            : NV * int(sizeof(T)) <= 8 ? 3
                                                       : 1;
 template <class T, int VEC, int NV, bool LAYER, bool POST>
-__global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(const __grid_constant__ Fwd a) {
-  __shared__ float red[4][WARPS];
+__global__ void __launch_bounds__(MAX_THREADS<VEC>, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(const __grid_constant__ Fwd a) {
+  __shared__ float red[4][WARPS<VEC>];
   using P = vec::Pack<T, VEC>;
   const int warps = blockDim.x >> 5;
   const int nvec = a.D / VEC;
@@ -102,7 +107,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(co
 #pragma unroll
           for (int j = 0; j < VEC; ++j) s += f[j];
         }
-      mean = block_sum(s, red[0], warps) / float(a.D);
+      mean = block_sum<WARPS<VEC>>(s, red[0], warps) / float(a.D);
       s = 0.f;
     }
 #pragma unroll
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(co
           s += c * c;
         }
       }
-    inv = rsqrtf(block_sum(s, red[1], warps) / float(a.D) + a.post_eps);
+    inv = rsqrtf(block_sum<WARPS<VEC>>(s, red[1], warps) / float(a.D) + a.post_eps);
     if (a.post_rstd && threadIdx.x == 0) {
       a.post_rstd[row] = inv;
       if (LAYER) a.post_mean[row] = mean;
@@ -177,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(co
       finish(i, v, u);
     }
   }
-  float total = block_sum(s, red[2], warps);
+  float total = block_sum<WARPS<VEC>>(s, red[2], warps);
   if (LAYER) {
     mean = total / float(a.D);
     s = 0.f;
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(THREADS, FWD_BLOCKS<T, VEC, NV>) fwd_kernel(co
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s += (f[j] - mean) * (f[j] - mean);
       }
-    total = block_sum(s, red[3], warps);
+    total = block_sum<WARPS<VEC>>(s, red[3], warps);
   }
   inv = rsqrtf(total / float(a.D) + a.eps);
   if (a.rstd && threadIdx.x == 0) {
@@ -241,6 +246,7 @@ struct Bwd {
 };
 
 // Sum over a group of `threads` threads of the block that meet at barrier `id`.
+template <int MOST>
 __device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int tid, int threads, int id) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -251,7 +257,7 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int tid, int
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
   float2 t = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < WARPS; ++i)
+  for (int i = 0; i < MOST; ++i)
     if (i < threads / 32) t.x += red[i].x, t.y += red[i].y;
   return t;
 }
@@ -263,13 +269,13 @@ __device__ __forceinline__ float2 group_sum2(float2 v, float2* red, int tid, int
 // the sums' join 10 -> 6.
 constexpr int GROUP_THREADS = 512;
 template <class T, int VEC, int NV, bool LAYER, bool POST>
-__global__ void __launch_bounds__(NV == 1 ? GROUP_THREADS : THREADS) bwd_kernel(const __grid_constant__ Bwd a) {
-  constexpr bool REG = NV == 1;
+__global__ void __launch_bounds__(VEC == 8 && NV == 1 ? GROUP_THREADS : MAX_THREADS<VEC>) bwd_kernel(const __grid_constant__ Bwd a) {
+  constexpr bool REG = VEC == 8 && NV == 1;
   // [slots][VEC][vectors]: value j of vector v at (slot * VEC + j) * nvec + v, so that neighbouring
   // threads are in neighbouring banks
   extern __shared__ float sums[];
   constexpr int GROUPS = REG ? GROUP_THREADS / 32 : 1;
-  __shared__ float2 red_all[GROUPS][2][2][WARPS];
+  __shared__ float2 red_all[GROUPS][2][2][WARPS<VEC>];
   using P = vec::Pack<T, VEC>;
   const int threads = a.group_threads;
   const int group = threadIdx.x / threads, tid = threadIdx.x - group * threads, bar = 1 + group;
@@ -344,7 +350,7 @@ __global__ void __launch_bounds__(NV == 1 ? GROUP_THREADS : THREADS) bwd_kernel(
           }
         }
       }
-      c = group_sum2(c, red[par][0], tid, threads, bar);
+      c = group_sum2<WARPS<VEC>>(c, red[par][0], tid, threads, bar);
       c.x /= float(a.D);
       c.y /= float(a.D);
     }
@@ -416,7 +422,7 @@ __global__ void __launch_bounds__(NV == 1 ? GROUP_THREADS : THREADS) bwd_kernel(
       }
     }
     if (POST) {
-      e = group_sum2(e, red[par][1], tid, threads, bar);
+      e = group_sum2<WARPS<VEC>>(e, red[par][1], tid, threads, bar);
       e.x /= float(a.D);
       e.y /= float(a.D);
     }
@@ -545,9 +551,12 @@ __global__ void __launch_bounds__(256) edge_kernel(const float* edge, T* dgate, 
   dgate[q * D + col] = vec::from_f<T>(s);
 }
 
-// Threads of a block: one for each vector of 8 values (wide) or each value, THREADS at most.
+// Threads of a row: one for each vector of 8 values (wide) or each value, up to a limit.  4096 bf16
+// rows of single values with both norms take 18 us at width 1001 with 256 threads and 25 with 512, at
+// 3585 83 and 61.
 static int threads_for(int64_t D, bool wide) {
-  return int(std::min<int64_t>(THREADS, ((wide ? D / 8 : D) + 31) / 32 * 32));
+  const int64_t most = wide || D <= 4 * THREADS ? THREADS : THREADS_NARROW;
+  return int(std::min<int64_t>(most, ((wide ? D / 8 : D) + 31) / 32 * 32));
 }
 
 // Calls f with (VEC, NV) as constants: the fewest vectors a thread that hold the row.
@@ -560,10 +569,9 @@ static void with_shape(int64_t D, bool wide, F f) {
     else if (nv <= 4) f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
     else f(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
   } else {
-    const int64_t nv = (D + THREADS - 1) / THREADS;
-    if (nv <= 4) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-    else if (nv <= 16) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-    else f(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+    if (D <= 4 * THREADS) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+    else if (D <= 8 * THREADS_NARROW) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
   }
 }
 
@@ -602,9 +610,9 @@ static void run_bwd(const Bwd& a, unsigned blocks, bool wide, bool layer, size_t
 
 static bool aligned(const torch::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
-// Widths are held in registers: 8 vectors of 8 a thread, or 32 single values where D is no multiple
+// Widths are held in registers: 8 vectors of 8 a thread, or 16 single values where D is no multiple
 // of 8 or a row does not start on 16 bytes.
-constexpr int64_t MAX_D = 8 * 8 * THREADS, MAX_D_NARROW = 32 * THREADS;
+constexpr int64_t MAX_D = 8 * 8 * THREADS, MAX_D_NARROW = 16 * THREADS_NARROW;
 constexpr size_t MAX_SUMS = 224 * 1024;  // bytes of shared memory for column sums
 
 }  // namespace bnorm
