@@ -157,9 +157,7 @@ def _cfg_from_hf(hc: Any) -> LMConfig:
         if (rope.get("rope_type") or rope.get("type")) == "dynamic":
             rope["original_max_position_embeddings"] = kw["n_ctx"]
         kw["rope_scaling"] = {k: v for k, v in rope.items() if v is not None}
-    part = rope.get("partial_rotary_factor") or getattr(hc, "partial_rotary_factor", None) or 1.0
-    if part != 1.0:
-        kw["rotary_dim"] = int(kw["d_head"] * part)
+    # A partial_rotary_factor stays where it is: the types converted here turn the whole head whatever it says.
     if mt in ("qwen2",):
         kw.update(architecture="qwen2", qkv_bias=True)
     elif mt in ("gemma2",):

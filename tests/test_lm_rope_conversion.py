@@ -1,0 +1,32 @@
+"""Rotary settings of Hugging Face configs, against transformers' own models; no device is needed."""
+
+import pytest
+import torch
+
+from saelens_b200.models.lm.hf import hooked_lm_from_hf
+
+transformers = pytest.importorskip("transformers")
+
+
+def converted(family, rope, **kw):
+    torch.manual_seed(0)
+    cfg = getattr(transformers, family + "Config")(
+        vocab_size=300, hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
+        num_key_value_heads=2, head_dim=16, max_position_embeddings=64, rope_parameters={"rope_theta": 10000.0, **rope}, **kw)
+    return getattr(transformers, family + "ForCausalLM")(cfg).eval()
+
+
+def check_same_logits(hf, length=60):
+    toks = torch.randint(0, 300, (2, length))
+    with torch.no_grad():
+        # fp32 on both sides, sums in another order: far below what a wrong angle moves (1e-3 and more)
+        assert torch.allclose(hooked_lm_from_hf(hf).eval()(toks), hf(input_ids=toks).logits, atol=1e-5, rtol=1e-5)
+
+
+@pytest.mark.parametrize("family", ["Llama", "Mistral", "Qwen2", "Gemma2"])
+@pytest.mark.parametrize("where", ["rope_parameters", "config"])
+def test_a_partial_factor_that_the_type_does_not_read(family, where):
+    part = {"partial_rotary_factor": 0.5}
+    hf = converted(family, {"rope_type": "default", **(part if where == "rope_parameters" else {})},
+                   **(part if where == "config" else {}))
+    check_same_logits(hf)
