@@ -23,9 +23,9 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict[str, Any] 
     base with the length, from `original_max_position_embeddings` on (`n_positions` is the length in
     use); "llama3" divides those that turn fewer than `low_freq_factor` times in the original context
     by `factor`, keeps those above `high_freq_factor` and blends between; "yarn" (Peng et al. 2023)
-    blends over pairs between `beta_slow` and `beta_fast` turns and puts `attention_factor` (0.1
-    ln(factor) + 1 unless given, or the ratio of 0.1 m ln(factor) + 1 for m = `mscale` and
-    `mscale_all_dim`) on cos and sin; "default" or None keeps them."""
+    blends over pairs between `beta_slow` and `beta_fast` turns (whole pairs, unless `truncate` is
+    false) and puts `attention_factor` (0.1 ln(factor) + 1 unless given, or the ratio of 0.1 m
+    ln(factor) + 1 for m = `mscale` and `mscale_all_dim`) on cos and sin; "default" or None keeps them."""
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary_frequencies: dim must be even and positive, got {dim}")
     if not base > 0:
@@ -61,8 +61,10 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: dict[str, Any] 
     def pair_of(turns: float) -> float:  # the pair that turns so often in the original context
         return dim * math.log(before / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    lo = max(math.floor(pair_of(float(s.get("beta_fast") or 32.0))), 0)
-    hi = min(math.ceil(pair_of(float(s.get("beta_slow") or 1.0))), dim - 1)
+    first, last = pair_of(float(s.get("beta_fast") or 32.0)), pair_of(float(s.get("beta_slow") or 1.0))
+    if s.get("truncate", True):
+        first, last = math.floor(first), math.ceil(last)
+    lo, hi = max(first, 0), min(last, dim - 1)
     ramp = ((i / 2 - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
 
     def stretch(m: float) -> float:

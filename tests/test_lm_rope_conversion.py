@@ -30,3 +30,11 @@ def test_a_partial_factor_that_the_type_does_not_read(family, where):
     hf = converted(family, {"rope_type": "default", **(part if where == "rope_parameters" else {})},
                    **(part if where == "config" else {}))
     check_same_logits(hf)
+
+
+YARN = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32}
+
+
+@pytest.mark.parametrize("more", [{"truncate": False}, {"truncate": True}, {"truncate": False, "beta_fast": 8.0, "beta_slow": 2.0}])
+def test_yarn_between_pairs(more):
+    check_same_logits(converted("Llama", {**YARN, **more}))
