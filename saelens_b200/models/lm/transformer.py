@@ -84,6 +84,22 @@ class LMConfig:
             raise ValueError(f"weight_quantization must be None or 'fp8', got {self.weight_quantization!r}")
         if self.rotary_dim is not None and not (2 <= self.rotary_dim <= self.d_head and self.rotary_dim % 2 == 0):
             raise ValueError(f"rotary_dim must be even and from 2 to d_head ({self.d_head}), got {self.rotary_dim}")
+        if self.positional == "rotary" and self.rotary_scaling() is not None:
+            self.rotary_frequencies(self.n_ctx)  # refuses what it cannot compute
+
+    def rotary_scaling(self) -> dict[str, Any] | None:
+        """How the context is stretched, as `ops.rotary_frequencies` takes it; None where it is not."""
+        s = self.rope_scaling or {}
+        kind = s.get("rope_type", s.get("type")) or "default"
+        if kind == "default":
+            return None
+        return {"original_max_position_embeddings": self.n_ctx, **s} if kind == "dynamic" else s
+
+    def rotary_frequencies(self, n_positions: int, device: Any = None) -> tuple[torch.Tensor, float]:
+        from saelens_b200.ops import rotary_frequencies
+
+        return rotary_frequencies(self.rotary_dim or self.d_head or 0, self.rotary_base, self.rotary_scaling(),
+                                  n_positions=n_positions, device=device)
 
     def to_dict(self) -> dict[str, Any]:
         return asdict(self)
@@ -680,17 +696,12 @@ class HookedLM(HookedRootModule):
         if cfg.positional != "rotary":
             return None
         dev = self.embed.weight.device
-        scaling = cfg.rope_scaling or {}
-        kind = scaling.get("rope_type", scaling.get("type")) or "default"
-        if kind != "default" or cfg.rotary_interleaved or cfg.rotary_dim not in (None, cfg.d_head):
+        scaling = cfg.rotary_scaling()
+        if scaling is not None or cfg.rotary_interleaved or cfg.rotary_dim not in (None, cfg.d_head):
             # only a dynamic stretch depends on the length
-            key = (dev, S if kind == "dynamic" else 0)
+            key = (dev, S if scaling is not None and scaling.get("rope_type", scaling.get("type")) == "dynamic" else 0)
             if self._freq is None or self._freq[0] != key:
-                from saelens_b200.ops import rotary_frequencies
-
-                scaling = {"original_max_position_embeddings": cfg.n_ctx, **scaling} if kind == "dynamic" else scaling
-                freq, factor = rotary_frequencies(cfg.rotary_dim or cfg.d_head or 0, cfg.rotary_base, scaling or None,
-                                                  n_positions=S, device=dev)
+                freq, factor = cfg.rotary_frequencies(S, dev)
                 self._freq = (key, RotaryFrequencies(freq, factor, cfg.rotary_interleaved))
             return self._freq[1]
         if self._rot is None or self._rot[0].shape[0] < S or self._rot[0].device != dev:

@@ -38,3 +38,33 @@ YARN = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 
 @pytest.mark.parametrize("more", [{"truncate": False}, {"truncate": True}, {"truncate": False, "beta_fast": 8.0, "beta_slow": 2.0}])
 def test_yarn_between_pairs(more):
     check_same_logits(converted("Llama", {**YARN, **more}))
+
+
+def tiny_config(**kw):
+    from saelens_b200.models.lm import preset_config
+
+    return preset_config("llama-3-8b", **{**dict(n_layers=1, d_model=64, n_heads=4, n_key_value_heads=2, d_mlp=128, d_vocab=300,
+                                                 n_ctx=64, d_head=16, dtype="float32"), **kw})
+
+
+@pytest.mark.parametrize("scaling,match", [
+    ({"rope_type": "linear", "factor": 0.5}, "factor"), ({"rope_type": "linear"}, "factor"),
+    ({"type": "yarn", "factor": 4.0}, "original_max"), ({"rope_type": "other", "factor": 2.0}, "unknown"),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 4.0, "original_max_position_embeddings": 32}, "high_freq"),
+])
+def test_a_scaling_is_checked_when_the_config_is_made(scaling, match):
+    with pytest.raises(ValueError, match=match):
+        tiny_config(rope_scaling=scaling)
+
+
+def test_scalings_that_are_not_used_or_need_no_length():
+    for kw in ({"rope_scaling": {"rope_type": "default"}}, {"rope_scaling": {}}, {"rope_scaling": {"rope_type": "dynamic", "factor": 2.0}},
+               {"positional": "standard", "rope_scaling": {"rope_type": "other"}}):
+        cfg = tiny_config(**kw)
+        assert cfg.rope_scaling == kw["rope_scaling"]
+    from saelens_b200.models.lm import HookedLM
+
+    torch.manual_seed(0)
+    lm = HookedLM(tiny_config(rope_scaling={"rope_type": "dynamic", "factor": 2.0}))
+    near, far = lm._rotary(64), lm._rotary(100)
+    assert torch.equal(near.freq, lm._rotary(10).freq) and (far.freq <= near.freq).all() and far.freq[-1] < near.freq[-1]
