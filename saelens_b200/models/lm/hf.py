@@ -153,8 +153,9 @@ def _cfg_from_hf(hc: Any) -> LMConfig:
         model_name=getattr(hc, "_name_or_path", mt) or mt, dtype="float32",
     )
     rope = dict(getattr(hc, "rope_scaling", None) or getattr(hc, "rope_parameters", None) or {})
-    if (rope.get("rope_type") or rope.get("type")) in ("linear", "dynamic", "llama3", "yarn"):
-        if (rope.get("rope_type") or rope.get("type")) == "dynamic":
+    kind = rope.get("rope_type") or rope.get("type") or "default"
+    if kind != "default":  # a kind that rotary_frequencies does not have is refused by LMConfig
+        if kind == "dynamic":
             rope["original_max_position_embeddings"] = kw["n_ctx"]
         kw["rope_scaling"] = {k: v for k, v in rope.items() if v is not None}
     # A partial_rotary_factor stays where it is: the types converted here turn the whole head whatever it says.

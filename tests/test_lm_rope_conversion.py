@@ -68,3 +68,21 @@ def test_scalings_that_are_not_used_or_need_no_length():
     lm = HookedLM(tiny_config(rope_scaling={"rope_type": "dynamic", "factor": 2.0}))
     near, far = lm._rotary(64), lm._rotary(100)
     assert torch.equal(near.freq, lm._rotary(10).freq) and (far.freq <= near.freq).all() and far.freq[-1] < near.freq[-1]
+
+
+def test_a_scaling_that_is_not_computed_is_refused():
+    """It was taken as no scaling at all."""
+    hf = converted("Llama", {"rope_type": "longrope", "factor": 2.0, "short_factor": [1.0] * 8, "long_factor": [2.0] * 8,
+                             "original_max_position_embeddings": 32})
+    with pytest.raises(ValueError, match="longrope"):
+        hooked_lm_from_hf(hf)
+
+
+@pytest.mark.parametrize("rope", [
+    {"rope_type": "default"}, {"rope_type": "linear", "factor": 4.0}, {"rope_type": "yarn", "factor": 4.0}, YARN,
+    {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0},
+    {"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 32},
+])
+@pytest.mark.parametrize("family", ["Llama", "Qwen2", "Gemma2"])
+def test_scalings_that_are_computed(family, rope):
+    check_same_logits(converted(family, rope), 100 if rope["rope_type"] == "dynamic" else 60)
