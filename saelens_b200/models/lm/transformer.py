@@ -308,23 +308,28 @@ class Norm(nn.Module):
 
 def _unwatched(m: nn.Module) -> bool:
     """Whether no hook of any kind watches the module."""
-    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+    hooks = nn.modules.module
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or hooks._global_forward_hooks or hooks._global_forward_pre_hooks
+                or hooks._global_backward_hooks or hooks._global_backward_pre_hooks)
 
 
-def _plain(hook: nn.Module) -> bool:
-    """Whether a hook point passes its tensor on unread (an SAE spliced in its place does not)."""
-    return isinstance(hook, HookPoint) and _unwatched(hook)
+def _stock(m: nn.Module | None, cls: type[nn.Module]) -> bool:
+    """Whether m does what `cls` does: not a subclass, not another module in its place, no `forward`
+    of the instance, no hook."""
+    return type(m) is cls and "forward" not in m.__dict__ and _unwatched(m)
 
 
-def _fuses_residual(x: torch.Tensor, out: torch.Tensor, post: Norm | None, hook_out: nn.Module, hook_stream: nn.Module,
-                    then: Norm, cfg: LMConfig) -> bool:
+def _fuses_residual(x: torch.Tensor, out: torch.Tensor, post: nn.Module | None, hook_out: nn.Module, hook_stream: nn.Module,
+                    then: nn.Module, cfg: LMConfig) -> bool:
     """Whether one kernel may do the residual update and the norms around it: inference on CUDA in a
-    type that the single norms run on, nothing reading in between."""
-    return (_native_ok(x) and x.dtype in (torch.bfloat16, torch.float32) and out.dtype == x.dtype == then.w.dtype
+    type that the single norms run on, nothing reading or computing something else in between."""
+    return (_stock(then, Norm) and (post is None or (_stock(post, Norm) and _stock(post.hook_normalized, HookPoint)))
+            and _stock(hook_out, HookPoint) and _stock(hook_stream, HookPoint)
+            and _native_ok(x) and x.dtype in (torch.bfloat16, torch.float32) and out.dtype == x.dtype == then.w.dtype
             and x.is_contiguous() and out.is_contiguous()
-            and 8 <= cfg.d_model <= 16384 and cfg.d_model % 8 == 0 and _plain(hook_out) and _plain(hook_stream)
-            and _unwatched(then)
-            and (post is None or (post.w.dtype == x.dtype and _unwatched(post) and _plain(post.hook_normalized))))
+            and 8 <= cfg.d_model <= 16384 and cfg.d_model % 8 == 0
+            and (post is None or post.w.dtype == x.dtype))
 
 
 def _act(name: str, x: torch.Tensor) -> torch.Tensor:
@@ -767,7 +772,7 @@ class HookedLM(HookedRootModule):
             if not _unwatched(blk):
                 pass
             elif i + 1 < end:
-                if _unwatched(self.blocks[i + 1]) and _plain(self.blocks[i + 1].hook_resid_pre):
+                if _unwatched(self.blocks[i + 1]) and _stock(self.blocks[i + 1].hook_resid_pre, HookPoint):
                     then = self.blocks[i + 1].ln1
             elif not stops and return_type is not None:
                 then = self.ln_final
