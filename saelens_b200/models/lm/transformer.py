@@ -769,14 +769,17 @@ class HookedLM(HookedRootModule):
         for i in range(start, end):
             blk, then = self.blocks[i], None
             # the norm that reads this block's stream next, when nothing can change the stream before it
-            if not _unwatched(blk):
+            if not _stock(blk, Block):
                 pass
             elif i + 1 < end:
-                if _unwatched(self.blocks[i + 1]) and _stock(self.blocks[i + 1].hook_resid_pre, HookPoint):
+                if _stock(self.blocks[i + 1], Block) and _stock(self.blocks[i + 1].hook_resid_pre, HookPoint):
                     then = self.blocks[i + 1].ln1
             elif not stops and return_type is not None:
                 then = self.ln_final
-            x, normed = blk(x, rot, normed, then) if then is not None else (blk(x, rot, normed), None)
+            if then is not None:
+                x, normed = blk(x, rot, normed, then)
+            else:
+                x, normed = blk(x, rot) if normed is None else blk(x, rot, normed), None
         if stops:
             return x
         if return_type is None:

@@ -69,6 +69,43 @@ def test_hooks_of_all_modules_are_not_passed(where, monkeypatch):
     assert lm_mod._fuses_residual(x, x, None, hook, hook, lm.ln_final, lm.cfg)
 
 
+class Twice(nn.Module):
+    """A block of a program's own."""
+
+    def __init__(self, block):
+        super().__init__()
+        self.block = block
+
+    def forward(self, x, rot):
+        return self.block(self.block(x, rot), rot)
+
+
+def replaced_blocks(lm):
+    toks = torch.randint(0, 300, (2, 9), device=lm.device)
+    args = []
+    handle = lm.blocks[1].register_forward_pre_hook(lambda m, a: args.append(len(a)))
+    with torch.no_grad():
+        lm(toks)
+        handle.remove()
+        assert args == [2]  # a hook of a block sees what a block was always called with
+        x = lm(toks, stop_at_layer=1)
+        want = lm.blocks[1](lm.blocks[1](x, lm._rotary(9)), lm._rotary(9))
+        lm.blocks[1] = Twice(lm.blocks[1])
+        assert torch.equal(lm(toks, stop_at_layer=2), want)
+        logits = lm.unembed(lm.ln_final(lm.blocks[2](want, lm._rotary(9))))
+        assert torch.equal(lm(toks), logits)
+
+
+def test_a_replaced_block():
+    replaced_blocks(tiny())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_a_replaced_block_on_cuda(dtype):
+    replaced_blocks(tiny(device="cuda", dtype=dtype))
+
+
 @gpu
 @pytest.mark.parametrize("preset,names", [("llama-3-8b", ["ln1", "ln2"]), ("gemma-2-9b", ["ln1_post", "ln2", "ln2_post"])])
 @pytest.mark.parametrize("replace", REPLACED)
