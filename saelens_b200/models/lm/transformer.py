@@ -329,7 +329,8 @@ def _fuses_residual(x: torch.Tensor, out: torch.Tensor, post: nn.Module | None, 
             and _native_ok(x) and x.dtype in (torch.bfloat16, torch.float32) and out.dtype == x.dtype == then.w.dtype
             and x.is_contiguous() and out.is_contiguous()
             and 8 <= cfg.d_model <= 16384 and cfg.d_model % 8 == 0
-            and (post is None or post.w.dtype == x.dtype))
+            # the kernel has one kind of norm and one way to weigh; each norm keeps its eps
+            and (post is None or (post.w.dtype == x.dtype and post.rms == then.rms and post.one_plus == then.one_plus)))
 
 
 def _act(name: str, x: torch.Tensor) -> torch.Tensor:
@@ -600,9 +601,10 @@ class Block(nn.Module):
             from saelens_b200 import ops
 
             stream, normed = ops.residual_norm(
-                x, out, then.w, then.b, kind="rms" if then.rms else "layer", eps=then.eps, one_plus=then.one_plus,
+                x, out, then.w, then.b, kind="rms" if then.rms else "layer", eps=then.eps,
+                one_plus=then.one_plus and then.rms,  # layer norms weigh with w whatever one_plus says
                 post_weight=None if post is None else post.w, post_bias=None if post is None else post.b,
-                gate=gate, scale=cfg.residual_scale, round_branch=True)
+                post_eps=None if post is None else post.eps, gate=gate, scale=cfg.residual_scale, round_branch=True)
             return stream, normed
         if post is not None:
             out = post(out)

@@ -69,6 +69,55 @@ def test_hooks_of_all_modules_are_not_passed(where, monkeypatch):
     assert lm_mod._fuses_residual(x, x, None, hook, hook, lm.ln_final, lm.cfg)
 
 
+def residual_norm_torch(x, branch, weight, bias, *, kind, eps, one_plus, post_weight, post_bias, gate, scale, round_branch,
+                        post_eps=None):
+    """`ops.residual_norm` by its definition, in fp32."""
+    def norm(t, w, b, e):
+        if kind == "layer":
+            t = t - t.mean(-1, keepdim=True)
+        t = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + e) * (w + 1 if one_plus else w)
+        return t if b is None else t + b
+
+    if post_weight is not None:
+        branch = norm(branch, post_weight, post_bias, eps if post_eps is None else post_eps)
+    stream = x + branch * scale
+    return stream, norm(stream, weight, bias, eps)
+
+
+@pytest.mark.parametrize("normalization", ["RMS", "LN"])
+@pytest.mark.parametrize("one_plus", [False, True])
+@pytest.mark.parametrize("change", [{}, {"eps": 0.5}, {"one_plus": True}, {"one_plus": False}])
+def test_the_fused_update_has_the_norms_settings(normalization, one_plus, change, monkeypatch):
+    """A post-norm's own eps, a layer norm that ignores `one_plus`, norms that weigh differently."""
+    from saelens_b200 import ops
+
+    lm = tiny("gemma-2-9b", normalization=normalization, rms_one_plus=one_plus)
+    blk, hook = lm.blocks[0], HookPoint()
+    for n, norm in enumerate((blk.ln1_post, blk.ln2)):
+        with torch.no_grad():
+            norm.w.normal_()
+            if norm.b is not None:
+                norm.b.normal_()
+    for name, value in change.items():
+        setattr(blk.ln1_post, name, value)
+    x, out = torch.randn(2, 5, 256), torch.randn(2, 5, 256)
+    with torch.no_grad():
+        stream = x + blk.ln1_post(out)
+        want = blk.ln2(stream)
+        # the update alone believes that its kernel runs, which is its definition here
+        fuses = lm_mod._fuses_residual
+        monkeypatch.setattr(lm_mod, "_native_ok", lambda t: True)
+        ok = fuses(x, out, blk.ln1_post, hook, hook, blk.ln2, lm.cfg)
+        monkeypatch.undo()
+        monkeypatch.setattr(lm_mod, "_fuses_residual", lambda *a: ok)
+        monkeypatch.setattr(ops, "residual_norm", residual_norm_torch)
+        got, normed = blk._join(x, out, blk.ln1_post, None, hook, hook, blk.ln2)
+        normed = blk.ln2(got) if normed is None else normed
+    # fp32 in two orders: 256 addends and a few products, 2^-24 each
+    assert torch.allclose(got, stream, atol=1e-4, rtol=1e-5) and torch.allclose(normed, want, atol=1e-4, rtol=1e-4)
+    assert ok or "one_plus" in change  # what may be fused still is
+
+
 class Twice(nn.Module):
     """A block of a program's own."""
 
