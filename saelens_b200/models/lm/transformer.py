@@ -26,7 +26,7 @@ from __future__ import annotations
 import contextlib
 
 import math
-from dataclasses import asdict, dataclass
+from dataclasses import asdict, dataclass, replace
 from typing import Any
 
 import torch
@@ -686,7 +686,7 @@ class HookedLM(HookedRootModule):
         from saelens_b200.models.lm.fp8 import quantize_lm_fp8
 
         quantize_lm_fp8(self)
-        self.cfg.weight_quantization = kind
+        self.cfg = replace(self.cfg, weight_quantization=kind)  # the config may be another model's too
         return self
 
     @property
