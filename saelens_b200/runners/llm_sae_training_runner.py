@@ -111,11 +111,23 @@ class LanguageModelSAETrainingRunner:
         self.model = None
         self.activations_store: Any = None
         if producer_side:
-            self.model = override_model if override_model is not None else self._load_model()
-            if getattr(self, "producer_tp_group", None) is not None:
+            tp_group = getattr(self, "producer_tp_group", None)
+            # a producer split over ranks is quantised after the split: each rank's weights have their own blocks
+            quantization = None
+            if override_model is not None:
+                self.model = override_model
+            elif tp_group is not None:
+                kw = dict(cfg.model_from_pretrained_kwargs or {})
+                quantization = kw.pop("weight_quantization", None)
+                self.model = self._load_model(kw)
+            else:
+                self.model = self._load_model()
+            if tp_group is not None:
                 from saelens_b200.models.lm.tp import shard_lm_tensor_parallel
 
-                shard_lm_tensor_parallel(self.model, self.producer_tp_group)  # Megatron split of the producer
+                shard_lm_tensor_parallel(self.model, tp_group)  # Megatron split of the producer
+                if quantization is not None:
+                    self.model.quantize_weights(quantization)
             if cfg.compile_llm:
                 self.model = torch.compile(self.model, mode=cfg.llm_compilation_mode)
             if self.streaming_mode:
@@ -182,11 +194,11 @@ class LanguageModelSAETrainingRunner:
     def _dp_rank(self) -> int:
         return dist.get_rank(self.dp_group) if self.dp_group is not None else 0
 
-    def _load_model(self) -> Any:
+    def _load_model(self, kwargs: dict[str, Any] | None = None) -> Any:
         from saelens_b200.models.lm.load_model import load_model
 
         return load_model(self.cfg.model_class_name, self.cfg.model_name, device=self.cfg.device,
-                          model_from_pretrained_kwargs=self.cfg.model_from_pretrained_kwargs)
+                          model_from_pretrained_kwargs=self.cfg.model_from_pretrained_kwargs if kwargs is None else kwargs)
 
     def _build_sae(self) -> TrainingSAE[Any]:
         cfg = self.cfg
