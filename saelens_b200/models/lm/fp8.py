@@ -62,6 +62,24 @@ class _TorchLinear(torch.autograd.Function):
         return dx.to(dy.dtype).view(*dy.shape[:-1], weight.shape[1]), None, None, None
 
 
+_CHECKED: dict[Any, int] = {}  # the backward pass that reads the status word at its end, for each word
+
+
+def _check_after_backward(status: Any) -> None:
+    """Read the status word once, when the backward pass under way has ended: a product of it that gave up
+    waiting raises there, not in the next forward pass.  (A capture reads nothing.)"""
+    task = torch._C._current_graph_task_id()
+    if _CHECKED.get(id(status)) == task:
+        return
+    _CHECKED[id(status)] = task
+
+    def check() -> None:
+        if not (status.tensor.is_cuda and torch.cuda.is_current_stream_capturing()):
+            status.check("producer LM backward")
+
+    torch.autograd.Variable._execution_engine.queue_callback(check)
+
+
 class Fp8Linear(nn.Module):
     """y = x W^T + b with W in e4m3, made from the weights (and biases) of one or several projections."""
 
@@ -104,7 +122,11 @@ class Fp8Linear(nn.Module):
             from saelens_b200 import ops
             from saelens_b200.models.lm.transformer import _status_for
 
-            return ops.linear_fp8(x, self.weight, self.scale, self.bias, status=_status_for(x))
+            status = _status_for(x)
+            y = ops.linear_fp8(x, self.weight, self.scale, self.bias, status=status)
+            if y.requires_grad:
+                y.register_hook(lambda _: _check_after_backward(status))
+            return y
         return _TorchLinear.apply(x, self.weight, self.scale, self.bias)
 
 
