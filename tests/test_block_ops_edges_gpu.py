@@ -1,0 +1,77 @@
+"""Calls of the block operators at their edges: derivatives that they do not have, gradients that lie
+oddly, batches without rows, results written in place, and column sums over many rows."""
+
+import pytest
+import torch
+
+from test_residual_norm_gpu import BF, EPS, F32, HF, chain_of, close, forward64, inputs, unit_back
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------ many rows
+MANY = [
+    # rows of 64: 15 groups a block, 2220 rows at once; sequences below, at and above a group's three rows
+    (64, F32, "layer", True, (2500, 2)), (64, BF, "rms", True, (1681, 3)), (64, HF, "rms", False, (721, 7)), (64, F32, "rms", True, (5, 1009)),
+    # 5 groups, 740 rows at once
+    (768, F32, "layer", True, (8, 513)), (768, BF, "layer", True, (684, 6)), (768, F32, "rms", True, (1026, 4)), (760, F32, "rms", False, (500, 9)),
+    # one group, sums in shared memory; sequences of a unit's rows, fewer and more
+    (4096, BF, "rms", True, (3, 1001)), (4096, BF, "layer", True, (300, 10)), (4096, F32, "rms", False, (273, 11)), (2056, F32, "layer", True, (600, 5)),
+    # single values, 256 and 512 threads
+    (1001, BF, "layer", True, (3, 1003)), (1001, F32, "rms", True, (375, 8)), (3001, F32, "rms", True, (429, 7)), (3001, BF, "layer", False, (5, 600)),
+]
+
+
+@pytest.mark.parametrize("d,dtype,kind,post,lead", MANY)
+@pytest.mark.parametrize("gate", [None, "channel", "sequence", "token"])
+def test_gradients_over_many_rows(d, dtype, kind, post, lead, gate):
+    """Several rows a unit: sums carried from row to row, buffers that alternate, sequences that begin
+    and end inside a unit, units that the last rows do not fill."""
+    from saelens_b200 import ops
+
+    layer, (b, s) = kind == "layer", lead
+    shape = {None: None, "channel": (), "sequence": (b, 1), "token": (b, s)}[gate]
+    v = {n: t.requires_grad_() for n, t in inputs(None, d, dtype, kind, post, shape, lead).items()}
+    scale = 1.0 if gate is None else -0.75
+    stream, normed = ops.residual_norm(**v, kind=kind, eps=EPS, scale=scale)
+    ds, dn = (torch.randn(*lead, d, device="cuda").to(dtype) for _ in range(2))
+    got = dict(zip(v, torch.autograd.grad((stream, normed), list(v.values()), (ds, dn))))
+    r = forward64(v, kind, False, scale, stored=stream)
+    f, dsd, dnd = r["f"], ds.double(), dn.double()
+    rows = (0, 1)
+    want, mags = {}, {}
+    want["weight"], mags["weight"] = (dnd * r["unit"]).sum(rows), (dnd.abs() * r["t_mag"]).sum(rows)
+    if layer:
+        want["bias"], mags["bias"] = dnd.sum(rows), dnd.abs().sum(rows)
+    pre, pre_mag = unit_back(dnd * r["w"], r["unit"], r["r"], layer)
+    pre_mag = pre_mag + r["r"] * r["t_mag"] * (dnd * r["w"] * r["t_mag"]).abs().mean(-1, keepdim=True)
+    g, g_mag = dsd + pre, dsd.abs() + pre_mag
+    want["x"], mags["x"] = g, g_mag
+    if post:
+        b_mag = r["b_unit"].abs() + (r["b_r"] * f["branch"].abs().mean(-1, keepdim=True) if layer else 0)
+    if gate is not None:
+        # from the branch itself: under a gate of 0 (randn gives one in 10^7 values) nothing of it is left in
+        # the stream's magnitude, while the gate's gradient is the rounded sums' product with it as ever
+        u_mag = b_mag * f["post_weight"].abs() + f.get("post_bias", r["u"] * 0).abs() if post else f["branch"].abs()
+        p, m = scale * g * r["u"], abs(scale) * g_mag * u_mag
+        if gate != "token":
+            p, m = (t.sum(rows if gate == "channel" else 1, keepdim=True) for t in (p, m))
+        want["gate"], mags["gate"] = p.reshape(v["gate"].shape), m.reshape(v["gate"].shape)
+    du, du_mag = r["g"] * g, r["g"].abs() * g_mag
+    if post:
+        want["post_weight"], mags["post_weight"] = (du * r["b_unit"]).sum(rows), (du_mag * b_mag).sum(rows)
+        if layer:
+            want["post_bias"], mags["post_bias"] = du.sum(rows), du_mag.sum(rows)
+        h, h_mag = du * f["post_weight"], du_mag * f["post_weight"].abs()
+        du, _ = unit_back(h, r["b_unit"], r["b_r"], layer)
+        du_mag = r["b_r"] * (h_mag + b_mag * (h_mag * b_mag).mean(-1, keepdim=True) * 2 + h_mag.mean(-1, keepdim=True))
+    want["branch"], mags["branch"] = du, du_mag
+    assert set(got) == set(want)
+    # a value's own roundings are those of the small cases; a column adds a unit's rows one by one (a
+    # 148th of all or 11 at most), 15 groups, 16 parts of at most 8 x 148 blocks and the 16 parts, a
+    # sequence that spans units one part for each
+    chain = 3 * chain_of(d) + max(b * s // 148 + 8, 11) + 15 + 8 * 148 // 16 + 16
+    for name in v:
+        close(got[name], want[name], mags[name], chain + (s if name == "gate" else 0), name)
+    again = torch.autograd.grad(ops.residual_norm(**v, kind=kind, eps=EPS, scale=scale), list(v.values()), (ds, dn))
+    assert all(torch.equal(got[n], t) for n, t in zip(v, again))  # the same bits again
