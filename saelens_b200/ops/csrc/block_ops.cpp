@@ -5,6 +5,7 @@
 #include "block_ops.h"
 
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "check.h"
 
@@ -27,10 +28,21 @@ torch::Tensor rows_of(const torch::Tensor& t) {
   return r.stride(1) == 1 || D == 1 ? r : r.contiguous();
 }
 
-// Backward passes of one order: a second one through them is refused, not silently zero.
+// Backward passes of one order: a second one through them is refused, not silently zero.  check_once sees
+// incoming gradients that have a graph; `once` marks gradients that depend on more than those, so
+// that a derivative of them, whatever the incoming ones, is an error when it is asked for.
 void check_once(const variable_list& grads, const char* name) {
   if (!at::GradMode::is_enabled()) return;
   for (const auto& g : grads) SB_CHECK(!wants_grad(g), name, " is differentiable once");
+}
+
+variable_list once(variable_list grads, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined())
+      g = (*std::make_shared<torch::autograd::DelayedError>(sb::detail::check_msg(name, " is differentiable once"), 1))(
+          {g.detach().requires_grad_()})[0];
+  return grads;
 }
 
 bool is_float(const torch::Tensor& t) {
@@ -133,7 +145,7 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     if (dpw) out[4] = *dpw;
     if (dpb) out[5] = *dpb;
     if (dg) out[6] = *dg;
-    return out;
+    return once(std::move(out), "residual_norm");
   }
 };
 

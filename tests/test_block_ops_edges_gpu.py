@@ -9,6 +9,27 @@ from test_residual_norm_gpu import BF, EPS, F32, HF, chain_of, close, forward64,
 pytestmark = pytest.mark.gpu
 
 
+# ------------------------------------------------------------------------------------ derivatives
+@pytest.mark.parametrize("name", ["x", "branch", "weight", "bias", "post_weight", "post_bias", "gate"])
+def test_the_gradient_of_the_norms_gradient_is_refused(name):
+    """The first gradient depends on every input, whether or not the incoming gradient does."""
+    from saelens_b200 import ops
+
+    v = inputs(5, 64, F32, "layer", True, ())
+    v[name].requires_grad_()
+    s, y = ops.residual_norm(**v, kind="layer")
+    (g,) = torch.autograd.grad(s.sum() + y.sum(), [v[name]], create_graph=True)
+    (want,) = torch.autograd.grad(sum(t.sum() for t in ops.residual_norm(**v, kind="layer")), [v[name]])
+    assert torch.equal(g.detach(), want)
+    with pytest.raises(RuntimeError, match="once"):
+        g.square().sum().backward()
+    # a loss that does not go through the first gradient is not concerned
+    s, y = ops.residual_norm(**v, kind="layer")
+    (g,) = torch.autograd.grad(y.sum(), [v[name]], create_graph=True)
+    (y.square().sum() + g.detach().sum()).backward()
+    assert torch.isfinite(v[name].grad).all()
+
+
 # ------------------------------------------------------------------------------------ many rows
 MANY = [
     # rows of 64: 15 groups a block, 2220 rows at once; sequences below, at and above a group's three rows
