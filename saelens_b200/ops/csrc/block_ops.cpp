@@ -19,6 +19,10 @@ using Opt = c10::optional<torch::Tensor>;
 bool wants_grad(const torch::Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants_grad(const Opt& t) { return t && t->requires_grad(); }
 
+// Forward-mode derivatives are not computed: an input's tangent is refused, not silently dropped.
+bool has_tangent(const torch::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const Opt& t) { return t && has_tangent(*t); }
+
 Opt opt(const torch::Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 
 // [..., D] as [rows, D] with contiguous rows: a view where the layout allows it.
@@ -240,6 +244,7 @@ torch::Tensor linear_fp8(const torch::Tensor& x, const torch::Tensor& weight, co
   SB_VALUE(x.dim() >= 1 && is_float(x) && x.size(-1) >= 1, "linear_fp8: x must be bf16, fp16 or fp32 [..., width]");
   SB_VALUE(weight.dim() == 2 && weight.scalar_type() == at::kFloat8_e4m3fn && weight.size(0) >= 1 && weight.size(1) == x.size(-1),
            "linear_fp8: the weight must be float8_e4m3fn [features, ", x.size(-1), "]");
+  SB_VALUE(!has_tangent(x) && !has_tangent(scale) && !has_tangent(bias), "linear_fp8 has no forward-mode derivative");
   if (at::GradMode::is_enabled()) {
     SB_VALUE(!scale.requires_grad() && !wants_grad(bias) && !weight.requires_grad(),
              "linear_fp8: the weight, its scales and the bias are frozen; only x has a gradient");
@@ -266,6 +271,9 @@ std::tuple<torch::Tensor, torch::Tensor> residual_norm(const torch::Tensor& x, c
   if (b) check(*b, "bias", true);
   if (post_w) check(*post_w, "post_weight", true);
   if (post_b) check(*post_b, "post_bias", true);
+  SB_VALUE(!has_tangent(x) && !has_tangent(branch) && !has_tangent(w) && !has_tangent(b) && !has_tangent(post_w) &&
+               !has_tangent(post_b) && !has_tangent(gate),
+           "residual_norm has no forward-mode derivative");
   auto vector = [](const Opt& t) { return t && !t->is_contiguous() ? Opt(t->contiguous()) : t; };
   const torch::Tensor wc = w.is_contiguous() ? w : w.contiguous();
   const Opt bc = vector(b), pw = vector(post_w), pb = vector(post_b);
@@ -311,6 +319,7 @@ std::tuple<torch::Tensor, Opt> rotary(const torch::Tensor& q, const Opt& k, cons
            "rotary: k does not match q");
   SB_VALUE(freq.dim() == 1 && freq.scalar_type() == at::kDouble && !freq.requires_grad() && freq.numel() >= 1 && 2 * freq.numel() <= d,
            "rotary: freq must be constant fp64 [rot / 2] with rot from 2 to ", d);
+  SB_VALUE(!has_tangent(q) && !has_tangent(k) && !has_tangent(freq), "rotary has no forward-mode derivative");
   Opt pos;
   if (positions) {
     const auto t = positions->scalar_type();

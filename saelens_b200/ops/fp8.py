@@ -105,7 +105,7 @@ def linear_fp8(
     x [..., K] bf16, fp16 or fp32; weight float8_e4m3fn [N, K] and scale [ceil(N / 128), ceil(K / 128)]
     from `quantize_fp8(w, 128)`; bias fp32 [N].  The weight, its scales and the bias are frozen; the
     gradient of x is the product with the weight's other side, its incoming gradient quantised the
-    same way (the quantisation of x counts as the identity).  Without `status` every call reads its
+    same way (the quantisation of x counts as the identity); tangents (forward mode) are refused.  Without `status` every call reads its
     own status word, which waits for the device; a program passes one word and checks it when it
     waits anyway (and has to under CUDA graph capture)."""
     if x.is_cuda and status is not None:  # checked where it is launched

@@ -50,7 +50,7 @@ def residual_norm(
     reads it as stored; `round_branch` also rounds the post-norm's output and the gated and scaled
     branch, as a program does that stores them.  Sums are 32-bit and deterministic.
 
-    Differentiable in all tensors (once).  D up to 16384 for rows of 16-byte vectors (D a multiple of
+    Differentiable in all tensors, once and backward (tangents are refused).  D up to 16384 for rows of 16-byte vectors (D a multiple of
     8, rows starting on 16 bytes), 8192 otherwise; with gradients the wanted column sums (one for
     each vector and a gate that rows share) of D fp32 have to fit 224 KB together."""
     if kind not in ("rms", "layer"):

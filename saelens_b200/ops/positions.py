@@ -96,7 +96,8 @@ def rotary(
     strides with contiguous channels (views of a fused projection); freq fp64 [rot / 2] on q's device
     (`rotary_frequencies`).  `positions` int64 or int32, [B, S] or what broadcasts to it, any value;
     without it token s is at offset + s.  Returns new tensors, or with `inplace` q and k themselves
-    (not under autograd).  Differentiable in q and k."""
+    (not under autograd).  Differentiable in q and k, any number of times; tangents (forward mode) are
+    refused."""
     if q.is_cuda:  # checked where it is launched
         out = load().rotary(q, k, freq, positions, offset, interleaved, factor, inplace)
         return out if k is not None else out[0]

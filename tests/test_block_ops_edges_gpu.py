@@ -10,6 +10,44 @@ pytestmark = pytest.mark.gpu
 
 
 # ------------------------------------------------------------------------------------ derivatives
+def forward_calls():
+    """Each operator as a function of one tensor, for each of its differentiable arguments."""
+    from saelens_b200 import ops
+
+    st = ops.StatusWord("cuda")
+    w, s = ops.quantize_fp8(torch.randn(128, 64, device="cuda"), 128)
+    x, a, v = torch.randn(3, 64, device="cuda"), torch.randn(3, 64, device="cuda"), torch.randn(64, device="cuda")
+    q, f = torch.randn(1, 3, 2, 64, device="cuda"), torch.ones(32, device="cuda", dtype=torch.float64)
+    norm = {"x": x, "branch": a, "weight": v, "bias": v, "post_weight": v, "post_bias": v, "gate": v}
+    calls = {"norm " + n: (lambda t, n=n: ops.residual_norm(**{**norm, n: t}, kind="layer"), norm[n]) for n in norm}
+    calls["linear x"] = (lambda t: ops.linear_fp8(t, w, s, status=st), x)
+    calls["linear x, own status"] = (lambda t: ops.linear_fp8(t, w, s), x)
+    calls["linear bias"] = (lambda t: ops.linear_fp8(x, w, s, t, status=st), torch.zeros(128, device="cuda"))
+    calls["linear scale"] = (lambda t: ops.linear_fp8(x, w, t, status=st), s)
+    calls["rotary q"] = (lambda t: ops.rotary(t, q, f), q)
+    calls["rotary k"] = (lambda t: ops.rotary(q, t, f), q)
+    calls["rotary freq"] = (lambda t: ops.rotary(q, None, t), f)
+    calls["rotary in place"] = (lambda t: ops.rotary(t, None, f, inplace=True), q.clone())
+    return calls
+
+
+CALLS = ["norm " + n for n in ("x", "branch", "weight", "bias", "post_weight", "post_bias", "gate")] + [
+    "linear x", "linear x, own status", "linear bias", "linear scale", "rotary q", "rotary k", "rotary freq", "rotary in place"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(name, grad):
+    """Forward-mode derivatives are not computed; a tangent may not be dropped without a word."""
+    import torch.autograd.forward_ad as fw
+
+    call, t = forward_calls()[name]
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        call(t)
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(fw.make_dual(t, torch.ones_like(t)))
+
+
 @pytest.mark.parametrize("name", ["x", "branch", "weight", "bias", "post_weight", "post_bias", "gate"])
 def test_the_gradient_of_the_norms_gradient_is_refused(name):
     """The first gradient depends on every input, whether or not the incoming gradient does."""
