@@ -679,6 +679,12 @@ void residual_norm_fwd(const torch::Tensor& x, const torch::Tensor& branch, cons
 // Whether the backward pass can hold `sums` column sums of width D.
 bool residual_norm_bwd_fits(int64_t D, int64_t sums) { return size_t(D) * sums * 4 <= bnorm::MAX_SUMS; }
 
+// Whether rows of width D are held by 16-byte vectors alone, and whether those of t can be read so.
+bool residual_norm_needs_vectors(int64_t D) { return D > bnorm::MAX_D_NARROW; }
+bool residual_norm_vectors(const torch::Tensor& t) {
+  return bnorm::aligned(t) && (t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0);
+}
+
 // Gradients of residual_norm_fwd.  d_stream / d_normed may be absent (no gradient).  Writes dx, and
 // where given dbranch, dw, db, dpost_w, dpost_b ([D] of x's type) and dgate (like gate).  gate_mode:
 // 0 none, 1 one gate row, 2 a gate row for gate_div consecutive rows, 3 a gate row for each row.
@@ -714,10 +720,9 @@ void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::
              "residual_norm: gate");
   SB_CHECK(gate || !dgate, "residual_norm: dgate without a gate");
   SB_CHECK((layer || (!db && !dpost_b)) && (post_w || (!dpost_w && !dpost_b)), "residual_norm: gradient of an absent vector");
-  const int64_t e = stream.element_size();
   bool wide = D % 8 == 0 && bnorm::aligned(stream) && bnorm::aligned(w) && bnorm::aligned(dx);
-  auto fits = [&](const torch::Tensor& t) { return bnorm::aligned(t) && (rows <= 1 || (t.stride(0) * e) % 16 == 0); };
-  wide = wide && fits(branch) && (!d_stream || fits(*d_stream)) && (!d_normed || fits(*d_normed));
+  wide = wide && residual_norm_vectors(branch) && (!d_stream || residual_norm_vectors(*d_stream)) &&
+         (!d_normed || residual_norm_vectors(*d_normed));
   for (const auto* t : {&post_w, &post_b, &gate, &dbranch, &dgate}) wide = wide && (!*t || bnorm::aligned(**t));
   SB_CHECK(D <= (wide ? bnorm::MAX_D : bnorm::MAX_D_NARROW), "residual_norm: width ", D, " is above ",
            wide ? bnorm::MAX_D : bnorm::MAX_D_NARROW);

@@ -127,7 +127,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     const auto& has = ctx->saved_data["has"].toTupleRef().elements();
     const int64_t div = args[0].toInt(), mode = args[1].toInt();
     const double scale = args[2].toDouble();
-    auto rows = [](const torch::Tensor& t) { return t.defined() ? Opt(rows_of(t)) : Opt(); };
+    // A gradient may be a view that starts anywhere (a slice of what a concatenation got).  Rows too wide for
+    // single values, which the forward pass took by 16-byte vectors, are copied then.
+    auto rows = [](const torch::Tensor& t) {
+      if (!t.defined()) return Opt();
+      const torch::Tensor r = rows_of(t);
+      return Opt(residual_norm_needs_vectors(r.size(1)) && !residual_norm_vectors(r) ? r.clone(at::MemoryFormat::Contiguous) : r);
+    };
     // needs_input_grad counts the tensors that were given
     size_t edge = 3;
     auto next_needed = [&](int i) { return has[i].toBool() && ctx->needs_input_grad(edge++); };

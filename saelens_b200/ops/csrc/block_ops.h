@@ -19,6 +19,8 @@ void residual_norm_fwd(const torch::Tensor& x, const torch::Tensor& branch, cons
                        bool round_branch, const torch::Tensor& stream, const torch::Tensor& normed,
                        const c10::optional<torch::Tensor>& stats);
 bool residual_norm_bwd_fits(int64_t D, int64_t sums);
+bool residual_norm_needs_vectors(int64_t D);
+bool residual_norm_vectors(const torch::Tensor& rows);
 void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::optional<torch::Tensor>& d_normed,
                        const torch::Tensor& stream, const torch::Tensor& branch, const torch::Tensor& w,
                        const c10::optional<torch::Tensor>& post_w, const c10::optional<torch::Tensor>& post_b,

@@ -68,6 +68,23 @@ def test_the_gradient_of_the_norms_gradient_is_refused(name):
     assert torch.isfinite(v[name].grad).all()
 
 
+# ------------------------------------------------------------------------------------ odd layouts, no rows
+@pytest.mark.parametrize("d", [8200, 16384])
+@pytest.mark.parametrize("start,wide", [(0, 3), (3, 5), (8, 8)])
+def test_wide_rows_whose_gradient_is_a_view(d, start, wide):
+    """What concatenation and padding send back: a narrowed view whose rows start anywhere."""
+    from saelens_b200 import ops
+
+    v = {n: t.requires_grad_() for n, t in inputs(3, d, BF, "rms", True, None).items()}
+    s, y = ops.residual_norm(**v, eps=EPS)
+    gs, gy = (torch.randn(3, d + wide + 3, device="cuda").to(BF)[:, start : start + d] for _ in range(2))
+    names = list(v.values())
+    for outs, grads in (((s, y), (gs, gy)), ((s,), (gs,)), ((y,), (gy,))):
+        got = torch.autograd.grad(outs, names, grads, retain_graph=True, allow_unused=True)
+        want = torch.autograd.grad(outs, names, [g.contiguous() for g in grads], retain_graph=True, allow_unused=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ------------------------------------------------------------------------------------ many rows
 MANY = [
     # rows of 64: 15 groups a block, 2220 rows at once; sequences below, at and above a group's three rows
