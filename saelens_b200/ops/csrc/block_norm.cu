@@ -713,8 +713,8 @@ void residual_norm_bwd(const c10::optional<torch::Tensor>& d_stream, const c10::
   SB_CHECK((gate_mode == 0) == !gate.has_value() && gate_mode >= 0 && gate_mode <= 3 && gate_div >= 1, "residual_norm: gate mode");
   if (gate)
     SB_CHECK(same(*gate) && gate->dim() == 2 && gate->size(1) == D && gate->is_contiguous() &&
-                 (rows == 0 || (rows - 1) / gate_div < gate->size(0)) &&
-                 (gate_mode != 1 || gate->size(0) == 1) && (gate_mode != 2 || gate->size(0) * gate_div == rows) &&
+                 (rows == 0 || (rows - 1) / gate_div < gate->size(0)) && (gate_mode != 1 || gate->size(0) == 1) &&
+                 (gate_mode != 2 || rows == 0 || gate->size(0) * gate_div == rows) &&
                  (gate_mode != 3 || (gate_div == 1 && gate->size(0) == rows)) &&
                  (!dgate || (same(*dgate) && dgate->sizes() == gate->sizes() && dgate->is_contiguous())),
              "residual_norm: gate");

@@ -85,6 +85,19 @@ def test_wide_rows_whose_gradient_is_a_view(d, start, wide):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("x,gate", [((2, 0), (2, 1)), ((2, 0), (2, 0)), ((0, 3), (0, 1)), ((0, 3), (0, 3)), ((0, 3), (1, 1)), ((2, 0), ()),
+                                    ((2, 0, 3), (2, 1, 1)), ((2, 0, 3), (2, 0, 1)), ((2, 3, 0), (2, 3, 1))])
+def test_gradients_of_a_gate_without_rows(x, gate):
+    from saelens_b200 import ops
+
+    v = {n: t.requires_grad_() for n, t in inputs(None, 64, F32, "rms", True, gate, x).items()}
+    s, y = ops.residual_norm(**v)
+    assert s.shape == y.shape == (*x, 64)
+    got = torch.autograd.grad((s.sum() + y.sum()), list(v.values()))
+    for name, g in zip(v, got):
+        assert g.shape == v[name].shape and (g == 0).all(), name
+
+
 # ------------------------------------------------------------------------------------ many rows
 MANY = [
     # rows of 64: 15 groups a block, 2220 rows at once; sequences below, at and above a group's three rows
