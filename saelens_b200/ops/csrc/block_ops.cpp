@@ -188,6 +188,12 @@ bool may_share(const torch::Tensor& q, const torch::Tensor& k) {
   return apart < d || apart > step - d;
 }
 
+// What is written in place counts as a change: autograd then notices where it had saved the old values.
+// (Tensors made in inference mode count nothing.)
+void changed(const torch::Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 std::tuple<torch::Tensor, torch::Tensor> turn(const torch::Tensor& q0, const torch::Tensor& k0, const torch::Tensor& freq,
                                               const Opt& pos, int64_t offset, bool interleaved, bool inverse, double factor) {
   const torch::Tensor q = last_contiguous(q0);
@@ -355,6 +361,8 @@ std::tuple<torch::Tensor, Opt> rotary(const torch::Tensor& q, const Opt& k, cons
       SB_VALUE(!may_share(q, *k), "rotary: in place, q and k must not share values");
     }
     rotary_fwd(q, k, f, pos, offset, interleaved, false, factor, q, k);
+    changed(q);
+    if (k) changed(*k);
     return {q, k};
   }
   if (grad) {

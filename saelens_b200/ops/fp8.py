@@ -85,6 +85,10 @@ def gemm_fp8(
         if out_dtype not in _FLOATS:
             raise ValueError(f"gemm_fp8: out_dtype must be bf16, fp16 or fp32, got {out_dtype}")
         out = torch.empty(M, b.shape[0], dtype=out_dtype, device=a.device)
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("gemm_fp8: out must not require a gradient, the product has none")
+    elif not out.is_inference():
+        torch.autograd.graph.increment_version(out)  # autograd notices where it had saved the old values
     st = status or StatusWord(a.device)
     load().gemm_fp8(a, a_scale, b, b_scale, bias, out, st.tensor)
     if status is None:

@@ -98,6 +98,39 @@ def test_gradients_of_a_gate_without_rows(x, gate):
         assert g.shape == v[name].shape and (g == 0).all(), name
 
 
+# ------------------------------------------------------------------------------------ in place
+def test_results_in_place_count_as_changes():
+    """A tensor that autograd saved and that an operator then overwrites is noticed."""
+    from saelens_b200 import ops
+
+    f = torch.ones(32, device="cuda", dtype=torch.float64)
+    w = torch.randn(64, device="cuda", requires_grad=True)
+    for one in (lambda q, k: q, lambda q, k: k):
+        q, k = torch.randn(1, 3, 2, 64, device="cuda"), torch.randn(1, 3, 2, 64, device="cuda")
+        y = (one(q, k) * w).sum()
+        ops.rotary(q, k, f, inplace=True)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+    a, sa = ops.quantize_fp8(torch.randn(4, 64, device="cuda"), 1)
+    b, sb = ops.quantize_fp8(torch.randn(64, 64, device="cuda"), 128)
+    out = torch.randn(4, 64, device="cuda")
+    y = (out * w).sum()
+    ops.gemm_fp8(a, sa, b, sb, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    with torch.inference_mode():  # such tensors count nothing
+        q = torch.randn(1, 3, 2, 64, device="cuda")
+        want = ops.rotary(q, None, f)
+        assert torch.equal(ops.rotary(q, None, f, inplace=True), want)
+    assert torch.equal(ops.rotary(want.clone(), None, f, inplace=True), ops.rotary(want, None, f))
+    ops.rotary(q, None, f, inplace=True)  # written outside as well, as before
+    leaf = torch.zeros(4, 64, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="out"):
+        ops.gemm_fp8(a, sa, b, sb, out=leaf)
+    with torch.no_grad():
+        ops.gemm_fp8(a, sa, b, sb, out=leaf)
+
+
 # ------------------------------------------------------------------------------------ many rows
 MANY = [
     # rows of 64: 15 groups a block, 2220 rows at once; sequences below, at and above a group's three rows
