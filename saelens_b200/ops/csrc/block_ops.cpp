@@ -7,6 +7,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 #include "check.h"
 
 namespace sb {
@@ -162,6 +166,24 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
 // ------------------------------------------------------------------------------ rotary
 torch::Tensor last_contiguous(const torch::Tensor& t) {
   return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+
+// Whether no value of t is there twice: from the least stride on, each dimension steps over all that the
+// ones before it span.  So it is in what slices, transposes and views leave of a whole tensor; other
+// layouts that hold each value once are rare, and refused with the rest.
+bool apart(const torch::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 0) return true;
+    if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+  }
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 1;
+  for (const auto& [stride, size] : dims) {
+    if (stride < span) return false;
+    span += (size - 1) * stride;
+  }
+  return true;
 }
 
 // Whether q and k of one storage may hold a value in common.  Views of one tensor have the same strides
@@ -351,9 +373,7 @@ std::tuple<torch::Tensor, Opt> rotary(const torch::Tensor& q, const Opt& k, cons
   if (inplace) {
     SB_VALUE(!grad, "rotary: not in place where gradients are wanted");
     auto check = [&](const torch::Tensor& t) {
-      bool ok = d <= 1 || t.stride(3) == 1;
-      for (int i = 0; i < 4; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) != 0);
-      SB_VALUE(ok, "rotary: in place needs contiguous channels and no value twice");
+      SB_VALUE((d <= 1 || t.stride(3) == 1) && apart(t), "rotary: in place needs contiguous channels and no value twice");
     };
     check(q);
     if (k) {
