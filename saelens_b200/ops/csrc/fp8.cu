@@ -1043,8 +1043,8 @@ static void product(const uint8_t* q, int64_t ldq, const float* scales, int64_t 
 static Prod prod_of(const Weight& w, int64_t M, const c10::optional<torch::Tensor>& bias, const torch::Tensor& out,
                     const torch::Tensor& status, const torch::Tensor& weight) {
   SB_CHECK(out.device() == weight.device() && out.dim() == 2 && out.size(0) == M && out.size(1) == w.F &&
-               (w.F <= 1 || out.stride(1) == 1) && float_type(out.scalar_type()),
-           "fp8 product: out must be bf16, fp16 or fp32 [rows, features] on the weight's device");
+               (w.F <= 1 || out.stride(1) == 1) && (M <= 1 || out.stride(0) >= w.F) && float_type(out.scalar_type()),
+           "fp8 product: out must be bf16, fp16 or fp32 [rows, features] on the weight's device, rows apart");
   if (bias)
     SB_CHECK(bias->device() == weight.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 &&
                  bias->size(0) == w.F && bias->is_contiguous(),

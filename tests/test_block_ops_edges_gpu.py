@@ -131,6 +131,22 @@ def test_results_in_place_count_as_changes():
         ops.gemm_fp8(a, sa, b, sb, out=leaf)
 
 
+def test_rows_of_out_that_overlap_are_refused():
+    from saelens_b200 import ops
+
+    a, sa = ops.quantize_fp8(torch.randn(4, 64, device="cuda"), 1)
+    b, sb = ops.quantize_fp8(torch.randn(96, 64, device="cuda"), 128)
+    buf = torch.zeros(4 * 96, device="cuda")
+    for out in (buf[:96].expand(4, 96), buf.as_strided((4, 96), (95, 1)), buf.as_strided((4, 96), (32, 1))):
+        with pytest.raises(RuntimeError, match="rows apart"):
+            ops.gemm_fp8(a, sa, b, sb, out=out)
+    assert (buf == 0).all()
+    want = ops.gemm_fp8(a, sa, b, sb, out_dtype=F32)
+    assert torch.equal(ops.gemm_fp8(a, sa, b, sb, out=buf.view(4, 96)), want)
+    one = buf[:96].expand(1, 96)
+    assert torch.equal(ops.gemm_fp8(a[:1], sa[:1], b, sb, out=one), ops.gemm_fp8(a[:1], sa[:1], b, sb, out_dtype=F32))
+
+
 # ------------------------------------------------------------------------------------ many rows
 MANY = [
     # rows of 64: 15 groups a block, 2220 rows at once; sequences below, at and above a group's three rows
