@@ -238,9 +238,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// Arrival on a barrier of either block of a pair, ordered within this block: the accumulator has been
-// read (tcgen05.wait::ld), and no other memory is handed over.  A cluster-wide release waits for
-// every access under way and took twice the time of the products.
+// Arrival on a barrier of either block of a pair, ordered within this block.  Across the pair it hands over
+// the accumulator, which has been read by then (tcgen05.wait::ld), and nothing else: row scales have a
+// barrier of their block's own.  A cluster-wide release waits for every access under way and took twice
+// the time of the products.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -626,7 +627,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
   uint64_t* empty = full + C::STAGES;                            // in each block
   uint64_t* tfull = empty + C::STAGES;                           // in each block
   uint64_t* tempty = tfull + 2;                                  // in the first block: both blocks' warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  // PAIR, in each block: its own warps have read a slot of row scales.  On one SM tempty says as much.
+  uint64_t* sfree = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sfree + C::RING);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -644,6 +647,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
       mbar_init(&tfull[s], 1);
       mbar_init(&tempty[s], PAIR ? 16 : 8);
     }
+    if (PAIR)
+      for (int s = 0; s < C::RING; ++s) mbar_init(&sfree[s], 8);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -684,6 +689,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
               break;
             }
             float* ss = sS + (it % C::RING) * 128;
+            if (PAIR && !wait_bar(&sfree[it % C::RING], ((it / C::RING) & 1) ^ 1, abort_flag, a.status, kTimeoutTmaProducer)) {
+              ok = false;
+              break;
+            }
             if (PAIR) {
               const uint32_t fb = mapa_shared(smem_u32(&full[s]), 0);
               if (cta == 0) mbar_arrive_expect_tx(&full[s], 2 * (C::STAGE + 512));
@@ -788,6 +797,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
           tmem_ld_32x32b_x32(at, r[0]);
         }
         const float sc = my_scale[g * 128] * __shfl_sync(0xffffffffu, wv, rb & 31);
+        const uint32_t scale_read = smem_u32(&sfree[g]);
         g = g + 1 == C::RING ? 0 : g + 1;
 #pragma unroll
         for (int h = 0; h < CHUNKS; ++h) {
@@ -806,6 +816,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1)
               tc_fence_after();
               tmem_ld_32x32b_x32(lanes + (c ^ 1) * C::BN, r[0]);
             }
+            if (PAIR && lane == 0) mbar_arrive_pair(scale_read);  // behind what the next block waits for
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[h * 32 + i] += __uint_as_float(r[h & 1][i]) * sc;
