@@ -31,7 +31,7 @@ namespace sb {
 namespace rotary {
 
 constexpr int THREADS = 128;
-constexpr int HEADS = 4;  // heads whose loads a thread has under way at once
+constexpr int HEADS = 4;  // heads of a thread at most, whose loads are under way at once
 
 struct Side {  // q or k
   const void* in;
@@ -52,8 +52,7 @@ struct Args {
   int64_t tokens, threads;  // threads: tokens * lanes * chunks of a head
   int S, d, rot;
   int chunks;  // of a head: those that turn, then those that pass through (two vectors each)
-  int lanes;   // threads that share a chunk's heads: lane l has heads l, l + lanes, ...
-  int copy;    // 1: the channels from rot on are written too (out of place)
+  int lanes;   // threads that share a chunk's heads: lane l has heads l, l + lanes, ..., HEADS at most
 };
 
 template <class T, int VEC, bool INTERLEAVED>
@@ -89,18 +88,15 @@ __global__ void __launch_bounds__(THREADS, 6) kernel(const __grid_constant__ Arg
   T* qo = static_cast<T*>(a.q.out) + b * a.q.out_b + s * a.q.out_s;
   T* ko = static_cast<T*>(a.k.out) + b * a.k.out_b + s * a.k.out_s;
   vec::Pack<T, VEC> u[HEADS], v[HEADS];
-  auto load = [&](int h0) {
 #pragma unroll
-    for (int n = 0; n < HEADS; ++n) {
-      const int h = h0 + n * a.lanes;
-      if (h < heads) {
-        const T* p = h < a.q.heads ? qi + h * a.q.in_h : ki + (h - a.q.heads) * a.k.in_h;
-        u[n].load(p + i0);
-        if (two) v[n].load(p + i1);
-      }
+  for (int n = 0; n < HEADS; ++n) {
+    const int h = lane + n * a.lanes;
+    if (h < heads) {
+      const T* p = h < a.q.heads ? qi + h * a.q.in_h : ki + (h - a.q.heads) * a.k.in_h;
+      u[n].load(p + i0);
+      if (two) v[n].load(p + i1);
     }
-  };
-  load(lane);
+  }
   float c[VEC], sn[VEC];
   if (turns) {
     int64_t p = a.pos0 + s;
@@ -116,41 +112,38 @@ __global__ void __launch_bounds__(THREADS, 6) kernel(const __grid_constant__ Arg
       sn[m] *= a.inverse ? -a.factor : a.factor;
     }
   }
-  for (int h0 = lane; h0 < heads; h0 += HEADS * a.lanes) {
-    if (h0 != lane) load(h0);
 #pragma unroll
-    for (int n = 0; n < HEADS; ++n) {
-      const int h = h0 + n * a.lanes;
-      if (h >= heads) break;
-      if (turns) {
-        float x[VEC], y[VEC];
-        u[n].unpack(x);
-        v[n].unpack(y);
-        if (INTERLEAVED) {
-          // the 2 VEC channels of (u, v) are VEC neighbouring pairs
-          auto at2 = [&](int m) -> float& { return m < VEC ? x[m < VEC ? m : 0] : y[m < VEC ? 0 : m - VEC]; };
+  for (int n = 0; n < HEADS; ++n) {
+    const int h = lane + n * a.lanes;
+    if (h >= heads) break;
+    if (turns) {
+      float x[VEC], y[VEC];
+      u[n].unpack(x);
+      v[n].unpack(y);
+      if (INTERLEAVED) {
+        // the 2 VEC channels of (u, v) are VEC neighbouring pairs
+        auto at2 = [&](int m) -> float& { return m < VEC ? x[m < VEC ? m : 0] : y[m < VEC ? 0 : m - VEC]; };
 #pragma unroll
-          for (int m = 0; m < VEC; ++m) {
-            float &A = at2(2 * m), &B = at2(2 * m + 1);
-            const float na = A * c[m] - B * sn[m];
-            B = B * c[m] + A * sn[m];
-            A = na;
-          }
-        } else {
-#pragma unroll
-          for (int m = 0; m < VEC; ++m) {
-            const float na = x[m] * c[m] - y[m] * sn[m];
-            y[m] = y[m] * c[m] + x[m] * sn[m];
-            x[m] = na;
-          }
+        for (int m = 0; m < VEC; ++m) {
+          float &A = at2(2 * m), &B = at2(2 * m + 1);
+          const float na = A * c[m] - B * sn[m];
+          B = B * c[m] + A * sn[m];
+          A = na;
         }
-        u[n].pack(x);
-        v[n].pack(y);
+      } else {
+#pragma unroll
+        for (int m = 0; m < VEC; ++m) {
+          const float na = x[m] * c[m] - y[m] * sn[m];
+          y[m] = y[m] * c[m] + x[m] * sn[m];
+          x[m] = na;
+        }
       }
-      T* o = h < a.q.heads ? qo + h * a.q.out_h : ko + (h - a.q.heads) * a.k.out_h;
-      u[n].store(o + i0);
-      if (two) v[n].store(o + i1);
+      u[n].pack(x);
+      v[n].pack(y);
     }
+    T* o = h < a.q.heads ? qo + h * a.q.out_h : ko + (h - a.q.heads) * a.k.out_h;
+    u[n].store(o + i0);
+    if (two) v[n].store(o + i1);
   }
 }
 
@@ -238,7 +231,8 @@ void rotary_fwd(const torch::Tensor& q, const c10::optional<torch::Tensor>& k, c
   a.S = int(S);
   a.d = int(d);
   a.rot = int(rot);
-  a.copy = (q.data_ptr() != q_out.data_ptr() || (k && k->data_ptr() != k_out->data_ptr())) ? 1 : 0;
+  // out of place the channels from rot on are written too
+  const bool copy = q.data_ptr() != q_out.data_ptr() || (k && k->data_ptr() != k_out->data_ptr());
   const int heads = a.q.heads + a.k.heads;
   if (a.tokens == 0 || heads == 0) return;
   // the widest vector that every part of a head and every stride is a multiple of
@@ -246,7 +240,7 @@ void rotary_fwd(const torch::Tensor& q, const c10::optional<torch::Tensor>& k, c
   while (vec > 1 && ((rot / 2) % vec || d % vec || !rotary::fits(q, vec) || !rotary::fits(q_out, vec) ||
                      (k && (!rotary::fits(*k, vec) || !rotary::fits(*k_out, vec)))))
     vec /= 2;
-  a.chunks = int((rot / 2) / vec + (a.copy ? ((d - rot) / vec + 1) / 2 : 0));
+  a.chunks = int((rot / 2) / vec + (copy ? ((d - rot) / vec + 1) / 2 : 0));
   // a thread turns its chunk in HEADS heads, in fewer where that leaves SMs short of threads
   const int64_t wave = 148 * 1024;
   int64_t lanes = (heads + rotary::HEADS - 1) / rotary::HEADS;
