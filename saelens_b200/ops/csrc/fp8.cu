@@ -292,7 +292,6 @@ struct Prod {
   int64_t ldo;
   int M, F, R;          // rows, features, length of the reduction
   int splits;           // parts of the reduction (the cluster's blocks)
-  int dependent;        // 1: launched while the quantisation before it may still run (not read on the device)
   int* status;
 };
 
@@ -997,7 +996,7 @@ static int splits_for(int64_t feature_tiles, int64_t reduction_blocks) {
 }
 
 template <int NT, bool FUSED, class TX, class TO>
-static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, Prod a, bool x_aligned, cudaStream_t st) {
+static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, Prod a, bool x_aligned, bool dependent, cudaStream_t st) {
   const int64_t tiles = (w.F + BLK - 1) / BLK;
   SB_CHECK(tiles < (1ll << 27), "fp8 product: size of the weight");
   const CUtensorMap tW = weight_map(w, BLK);
@@ -1005,7 +1004,7 @@ static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& 
   a.splits = splits_for(tiles, (w.R + BLK - 1) / BLK);
   auto go = [&](auto aligned, auto mn) {
     launch<few_rows_kernel<NT, FUSED, decltype(aligned)::value, decltype(mn)::value, TX, TO>>(
-        dim3(unsigned(tiles * a.splits)), threads, smem, a.splits, a.dependent, st, tW, tX, tS, a);
+        dim3(unsigned(tiles * a.splits)), threads, smem, a.splits, dependent, st, tW, tX, tS, a);
   };
   if constexpr (FUSED) {
     if (!x_aligned) {
@@ -1017,7 +1016,7 @@ static void few_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& 
 }
 
 template <bool PAIR, int BN, class TO>
-static void many_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a, cudaStream_t st) {
+static void many_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap& tS, const Prod& a, bool dependent, cudaStream_t st) {
   using C = Many<PAIR, BN>;
   const int64_t tiles = ((a.M + C::BM - 1) / C::BM) * ((w.F + C::BN - 1) / C::BN);
   SB_CHECK(tiles < (1ll << 30), "fp8 product: too many tiles");
@@ -1025,29 +1024,30 @@ static void many_rows(const Weight& w, const CUtensorMap& tX, const CUtensorMap&
   const dim3 grid{unsigned(PAIR ? 2 * std::min<int64_t>(tiles, sms / 2) : std::min<int64_t>(tiles, sms))};
   const CUtensorMap tW = weight_map(w, C::W_ROWS);
   const int cluster = PAIR ? 2 : 1;
-  if (w.mn) launch<many_rows_kernel<PAIR, BN, true, TO>>(grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
-  else launch<many_rows_kernel<PAIR, BN, false, TO>>(grid, MANY_THREADS, C::SMEM, cluster, a.dependent, st, tW, tX, tS, a);
+  if (w.mn) launch<many_rows_kernel<PAIR, BN, true, TO>>(grid, MANY_THREADS, C::SMEM, cluster, dependent, st, tW, tX, tS, a);
+  else launch<many_rows_kernel<PAIR, BN, false, TO>>(grid, MANY_THREADS, C::SMEM, cluster, dependent, st, tW, tX, tS, a);
 }
 
 // Quantised rows (uint8 [M, R] with row stride ldq) and their scales ([blocks][lds]) times the weight.
+// `dependent`: launched right behind the kernel that quantises them, which may still run.
 template <class TO>
-static void product(const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, const Weight& w, const Prod& a, cudaStream_t st) {
+static void product(const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, const Weight& w, const Prod& a, bool dependent, cudaStream_t st) {
   const int box = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= FEW ? 64 : 128;
   const CUtensorMap tX = make_tmap_2d(q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.M, w.R, ldq, box, BLK, CU_TENSOR_MAP_SWIZZLE_128B);
   const CUtensorMap tS = make_tmap_2d(scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, (w.R + BLK - 1) / BLK, a.M, lds * 4, 1, box,
                                       CU_TENSOR_MAP_SWIZZLE_NONE);
-  if (a.M <= 16) few_rows<16, false, float, TO>(w, tX, tS, a, true, st);
-  else if (a.M <= 32) few_rows<32, false, float, TO>(w, tX, tS, a, true, st);
-  else if (a.M <= FEW) few_rows<64, false, float, TO>(w, tX, tS, a, true, st);
+  if (a.M <= 16) few_rows<16, false, float, TO>(w, tX, tS, a, true, dependent, st);
+  else if (a.M <= 32) few_rows<32, false, float, TO>(w, tX, tS, a, true, dependent, st);
+  else if (a.M <= FEW) few_rows<64, false, float, TO>(w, tX, tS, a, true, dependent, st);
   else {
     const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     // While one wave of SMs holds all tiles, the time is that of one tile: 0.37 us a block of 128 for 128
     // features, 0.49 for 256, 0.54 for a pair's (333 x 5120 -> 7168: 44, 29 and 31 us).  Beyond, a pair's
     // tile costs least for its size (2048 x 4096 -> 14336: 176, 146 and 137 us).
     const int64_t m = (a.M + 127) / 128;
-    if (m * ((w.F + 127) / 128) <= sms) many_rows<false, 128, TO>(w, tX, tS, a, st);
-    else if (m * ((w.F + 255) / 256) <= sms) many_rows<false, 256, TO>(w, tX, tS, a, st);
-    else many_rows<true, 256, TO>(w, tX, tS, a, st);
+    if (m * ((w.F + 127) / 128) <= sms) many_rows<false, 128, TO>(w, tX, tS, a, dependent, st);
+    else if (m * ((w.F + 255) / 256) <= sms) many_rows<false, 256, TO>(w, tX, tS, a, dependent, st);
+    else many_rows<true, 256, TO>(w, tX, tS, a, dependent, st);
   }
 }
 
@@ -1080,7 +1080,7 @@ static void linear_t(const torch::Tensor& x, const Weight& w, Prod a, cudaStream
   if (a.M <= FUSED_ROWS) {
     a.x = x.data_ptr();
     a.ldx = x.stride(0);
-    few_rows<16, true, T, T>(w, CUtensorMap{}, CUtensorMap{}, a, rows_aligned(x), st);
+    few_rows<16, true, T, T>(w, CUtensorMap{}, CUtensorMap{}, a, rows_aligned(x), false, st);
     return;
   }
   const int64_t ldq = up(w.R, 16), lds = up(a.M, 4), RB = (w.R + BLK - 1) / BLK;
@@ -1090,8 +1090,8 @@ static void linear_t(const torch::Tensor& x, const Weight& w, Prod a, cudaStream
   uint8_t* q = held.data_ptr<uint8_t>();
   float* s = reinterpret_cast<float*>(q + values);
   quantize_rows(x, q, ldq, s, lds, st);
-  a.dependent = 1;  // the quantisation itself began after everything before it had ended
-  product<T>(q, ldq, s, lds, w, a, st);
+  // dependent: the quantisation itself began after everything before it had ended
+  product<T>(q, ldq, s, lds, w, a, true, st);
 }
 
 }  // namespace fp8
@@ -1169,9 +1169,9 @@ void gemm_fp8(const torch::Tensor& a, const torch::Tensor& a_scale, const torch:
   fp8::bind_context(a);
   auto st = at::cuda::getCurrentCUDAStream();
   const uint8_t* q = static_cast<const uint8_t*>(a.data_ptr());
-  if (out.scalar_type() == at::kBFloat16) fp8::product<__nv_bfloat16>(q, ldq, sp, lds, w, p, st);
-  else if (out.scalar_type() == at::kHalf) fp8::product<__half>(q, ldq, sp, lds, w, p, st);
-  else fp8::product<float>(q, ldq, sp, lds, w, p, st);
+  if (out.scalar_type() == at::kBFloat16) fp8::product<__nv_bfloat16>(q, ldq, sp, lds, w, p, false, st);
+  else if (out.scalar_type() == at::kHalf) fp8::product<__half>(q, ldq, sp, lds, w, p, false, st);
+  else fp8::product<float>(q, ldq, sp, lds, w, p, false, st);
 }
 
 }  // namespace sb
