@@ -121,8 +121,9 @@ __device__ __forceinline__ float half_warp_most(const float (&v)[8]) {
 }
 
 // Rows: a half-warp quantises a row's 128 values, 8 a lane; 16 rows a block, PER blocks of 128 a
-// half-warp (all loads issued before the first maximum).  Memory-bound: 2 bytes read and 1 written
-// a value.
+// half-warp (all loads issued before the first maximum).  2 bytes are read and 1 written a value, but issue
+// slots bind before memory does: 8192 x 4096 values in 26 us at 66% of the issue slots (15 us of bytes at
+// the copy rate), 2048 x 14336 in 23 (13).
 template <class T, bool ALIGNED, int PER>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t ldx, int64_t M, int64_t K,
                                                             uint8_t* __restrict__ q, int64_t ldq,
@@ -301,9 +302,10 @@ struct Prod {
 // features and a part of the reduction; the blocks of a cluster hold the parts of the same features.
 // Column c of the sums belongs to block c % splits: every block writes its part of it there, over
 // distributed shared memory, and after one cluster barrier the owner adds the parts in block order.
-// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)  One row 4096 ->
-// 6144 8.0 us, 24 rows 14336 -> 4096 18.0 with their quantisation (25 and 59 MB of weight: 3.9 and 9.0
-// us at the copy rate); what remains is launch, the first bytes' latency and the cluster's barrier.
+// (Reading the parts instead took two barriers and a remote round trip, 3.3 us of 13.)  With launches
+// queued one row 4096 -> 6144 takes 10.4 us and 24 rows 14336 -> 4096 18.6 (25 and 59 MB of weight: 3.9 and
+// 9.0 us at the copy rate).  The 24 rows' quantisation hides beside the product, which takes 18.2 by itself,
+// 3.2 TB/s with 1.7 of its blocks an SM side by side.
 //   warp 0      weight tiles by TMA (and x tiles and scales, unless they are quantised here)
 //   warp 1      tcgen05.mma, 4 a block of 128
 //   warps 2..5  scaled sums in registers: a feature a thread, NT columns
@@ -550,7 +552,8 @@ __global__ void __launch_bounds__(FUSED ? 320 : 192, 2)
 // reduction goes to one of two TMEM accumulators, and the hand-over between products and sums is what
 // a block costs: 840 cycles a pair's, of which the products are 541 (without any scaling 690).  Under
 // sustained load the 1 kW limit binds: 77% of the same kernel's rate without scales.  8192 x 4096 ->
-// 28672 in 0.91 ms of products (2.1 PFLOP/s), 2048 x 4096 -> 14336 in 0.135 (1.8).
+// 28672 takes 0.91 ms by itself (2.1 PFLOP/s) and 1.05 under a long load (1.54 GHz at that limit), 2048 x
+// 4096 -> 14336 0.131 and 0.145, with row scales and weight scales applied, rows quantised before.
 //   warps 0..7   scaled sums in registers: a row a thread, half of the tile's features (warps 0-3 the first)
 //   warp 8       TMA;  warp 9  tcgen05.mma (in the pair's first block);  warps 10, 11 only give up registers
 template <bool PAIR, int BN_>
