@@ -1,4 +1,4 @@
-"""8-bit weights of the producer LM as a program reaches them; no device is needed."""
+"""8-bit weights of the producer LM as a program reaches them."""
 
 import pytest
 import torch
@@ -63,3 +63,41 @@ def test_a_wait_that_ran_out_in_a_backward_pass_raises_there(monkeypatch):
         assert _Fake.ran == 4 and len(read) == 1 and int(status.tensor) == 0  # one read for the whole pass
     with torch.no_grad():
         lm.blocks[0].mlp(x)
+
+
+@pytest.mark.gpu
+def test_a_backward_pass_on_cuda_reads_its_status():
+    """The word is read at the end of the pass, whichever thread ends it, and not under capture."""
+    from saelens_b200.models.lm import transformer as lm_mod
+    from saelens_b200.ops.status import KernelTimeoutError
+
+    lm = HookedLM(preset_config("llama-3-8b", **{**TINY, "dtype": "bfloat16"}), device="cuda").quantize_weights()
+    mlp = lm.blocks[0].mlp
+    x = torch.randn(2, 40, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    status = lm_mod._status_for(x)
+
+    def gradient():
+        return torch.autograd.grad(mlp(x).float().square().sum(), x)[0]
+
+    want = gradient()
+    y = mlp(x).float().square().sum()
+    status.tensor.fill_(2)  # as a wait that ran out writes it
+    with pytest.raises(KernelTimeoutError, match="backward"):
+        torch.autograd.grad(y, x)
+    assert status.code() == 0 and torch.equal(gradient(), want)
+    del y  # autograd ties a leaf to the stream of a graph that lives, which a capture may not join
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gradient()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = gradient()
+    for _ in range(2):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+        graph.replay()
+        assert torch.equal(held, gradient())
+    status.check()
