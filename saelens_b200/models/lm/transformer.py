@@ -306,18 +306,17 @@ class Norm(nn.Module):
         return self.hook_normalized(y.to(x.dtype))
 
 
-def _unwatched(m: nn.Module) -> bool:
-    """Whether no hook of any kind watches the module."""
-    hooks = nn.modules.module
-    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
-                or hooks._global_forward_hooks or hooks._global_forward_pre_hooks
-                or hooks._global_backward_hooks or hooks._global_backward_pre_hooks)
+_MODULE_HOOKS = nn.modules.module  # hooks of all modules are globals there
 
 
 def _stock(m: nn.Module | None, cls: type[nn.Module]) -> bool:
     """Whether m does what `cls` does: not a subclass, not another module in its place, no `forward`
-    of the instance, no hook."""
-    return type(m) is cls and "forward" not in m.__dict__ and _unwatched(m)
+    of the instance, no hook of its own or of all modules.  (Called a dozen times a block.)"""
+    if type(m) is not cls:
+        return False
+    d, g = m.__dict__, _MODULE_HOOKS
+    return not ("forward" in d or d["_forward_hooks"] or d["_forward_pre_hooks"] or d["_backward_hooks"] or d["_backward_pre_hooks"]
+                or g._global_forward_hooks or g._global_forward_pre_hooks or g._global_backward_hooks or g._global_backward_pre_hooks)
 
 
 def _fuses_residual(x: torch.Tensor, out: torch.Tensor, post: nn.Module | None, hook_out: nn.Module, hook_stream: nn.Module,
